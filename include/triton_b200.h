@@ -267,6 +267,130 @@ typedef struct {
 size_t tb200_attention_bwd_workspace_bytes(const tb200_attention_bwd_args* args);
 int tb200_attention_bwd(const tb200_attention_bwd_args* args, void* stream);
 
+/* ---------------------------------------------------------------- paged KV cache ---- */
+/*
+ * A paged cache is two pools of pages, keys and values, each an array [n_pages][page_size][kv_heads][head_dim] seen
+ * through three element strides (page, token, head; the head_dim values of a row are contiguous), so pages may lie token
+ * by token or head by head in memory. page_table: int32 [batch][max_pages] (table_stride elements between rows), the pages
+ * of a sequence in order; seq_lens: int32 [batch], its length in tokens. Position p of sequence b is token p % page_size
+ * of page page_table[b][p / page_size]. Lengths live on the device and are not known to the host: a length is taken as
+ * at most max_pages * page_size and at least 0, and a page outside [0, n_pages) is never accessed - it reads as a page
+ * of zeros and is not written.
+ * cache_dtype: `dtype`, or TB200_E4M3 with k_scale / v_scale (float, *_scale_n = 1 for the whole pool or kv_heads for one
+ * per head; a cached value stands for value * scale).
+ * None of these entry points has a counterpart in the reference; they continue tb200_attention_fwd (grouped heads, packed
+ * sequences, cached keys) for serving.
+ */
+
+/*
+ * Rotates `tokens` packed rows of queries and keys by their positions and appends keys and values to the cache.
+ * Token t belongs to the sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1] (int32 [batch + 1]; NULL: one token per
+ * sequence, tokens == batch) and has position seq_lens[b] - (cu_seqlens[b + 1] - t): seq_lens counts the new tokens.
+ * Rotation of the first rotary_dim columns by row `position` of cos and sin (float [n_positions][rotary_dim / 2],
+ * rot_stride elements between rows): (x, y) -> (x cos - y sin, y cos + x sin) for the pairs (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved; the other columns are copied. cos == NULL: no rotation. Arithmetic in fp32, one
+ * rounding; to e4m3 round to nearest even, saturating.
+ * q (with q_out) may be NULL; k_out (the rotated keys, packed) may be NULL; q_out == q and k_out == k are allowed.
+ * Tokens at or past cu_seqlens[batch]: nothing is written. A position below 0, at or past n_positions, or past the page
+ * table: the rows of q_out and k_out are zeros, the cache is left alone.
+ * head_dim 64, 128 or 256; rotary_dim a multiple of 16, at most head_dim; dtype TB200_BF16 or TB200_F16. All bases 16-byte
+ * aligned, all strides multiples of 8 elements (an e4m3 cache: 8-byte aligned, multiples of 8).
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  const float* cos;
+  const float* sin;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t tokens, batch, heads, kv_heads;
+  int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok, v_stride_head;
+  int64_t qo_stride_tok, qo_stride_head, ko_stride_tok, ko_stride_head;
+  int64_t kc_stride_page, kc_stride_tok, kc_stride_head, vc_stride_page, vc_stride_tok, vc_stride_head;
+  int64_t table_stride, rot_stride;
+  int64_t n_pages, max_pages, n_positions;
+  int32_t page_size, head_dim, rotary_dim, interleaved;
+  int32_t dtype, cache_dtype, k_scale_n, v_scale_n;
+} tb200_kv_append_args;
+int tb200_kv_append(const tb200_kv_append_args* args, void* stream);
+
+/*
+ * Attention of one new token per sequence over the cache: o[b, h] = softmax_j(sm_scale q[b, h] . k_j) v_j over the
+ * seq_lens[b] cached positions j of kv head h / (heads / kv_heads). lse (may be NULL): float [batch][heads], base-2
+ * log-sum-exp of the scaled scores. A sequence of length 0 gives o = 0 and lse = -inf.
+ * q, o: [batch][heads][head_dim] with element strides (multiples of 8; bases 16-byte aligned). Caches 16-byte aligned with
+ * strides that are multiples of 16 bytes. head_dim 64, 128 or 256; dtype TB200_BF16 or TB200_F16; sm_scale > 0.
+ * workspace: tb200_attention_decode_workspace_bytes(args) bytes, 16-byte aligned, contents free before and after; calls that
+ * may run at the same time need workspaces of their own.
+ */
+typedef struct {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const float* k_scale;
+  const float* v_scale;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t batch, heads, kv_heads;
+  int64_t q_stride_b, q_stride_head, o_stride_b, o_stride_head;
+  int64_t kc_stride_page, kc_stride_tok, kc_stride_head, vc_stride_page, vc_stride_tok, vc_stride_head;
+  int64_t table_stride, n_pages, max_pages;
+  int32_t page_size, head_dim, dtype, cache_dtype, k_scale_n, v_scale_n;
+  float sm_scale;
+  int32_t reserved;
+} tb200_attention_decode_args;
+size_t tb200_attention_decode_workspace_bytes(const tb200_attention_decode_args* args);
+int tb200_attention_decode(const tb200_attention_decode_args* args, void* stream);
+
+/*
+ * Attention of packed sequences of different lengths with grouped heads: query i of sequence b (n_q queries, n_k keys) sees
+ * the keys j <= i + n_k - n_q when causal (the last query sees every key), all of them otherwise; query head h reads kv
+ * head h / (heads / kv_heads). A query that sees no key gets o = 0 and lse = -inf.
+ * q, o: [tokens_q][heads][head_dim] and lse (may be NULL): float [tokens_q][heads], sequence b in rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (int32 [batch + 1]); rows outside every sequence are not written.
+ * page_size == 0: k, v are [tokens_k][kv_heads][head_dim], sequence b in rows cu_seqlens_k[b] .. cu_seqlens_k[b + 1].
+ * page_size > 0 (a multiple of 8): k, v are the two pools of a paged cache of `dtype` elements, n_k = seq_lens[b].
+ * No sequence's output depends on the rows of another, whatever those hold; a NaN or infinity in v makes the rows of its
+ * own sequence undefined, those that the mask keeps from it included (0 * inf).
+ * head_dim 64, 128 or 256; dtype TB200_BF16 or TB200_F16; sm_scale > 0; bases 16-byte aligned, strides (elements, at least
+ * head_dim) multiples of 8. workspace: tb200_attention_varlen_workspace_bytes(args) bytes, 32-byte aligned, contents free
+ * before and after; calls that may run at the same time need workspaces of their own.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_seqlens_k;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t tokens_q, tokens_k, batch, heads, kv_heads;
+  int64_t q_stride_tok, q_stride_head, o_stride_tok, o_stride_head;
+  int64_t k_stride_page, k_stride_tok, k_stride_head, v_stride_page, v_stride_tok, v_stride_head;
+  int64_t table_stride, n_pages, max_pages;
+  int32_t page_size, head_dim, dtype, causal;
+  float sm_scale;
+  int32_t reserved;
+} tb200_attention_varlen_args;
+size_t tb200_attention_varlen_workspace_bytes(const tb200_attention_varlen_args* args);
+int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* args, void* stream);
+
 /* ---------------------------------------------------------------- MoE routing ------ */
 /* Paths below are inside python/triton_kernels/triton_kernels/ of the reference. */
 

@@ -80,6 +80,40 @@ class AttentionBwdArgs(Structure):
     ]
 
 
+class KvAppendArgs(Structure):
+    _fields_ = [(n, c_void_p) for n in (
+        "q", "k", "v", "q_out", "k_out", "k_cache", "v_cache", "page_table", "seq_lens", "cu_seqlens", "cos", "sin",
+        "k_scale", "v_scale")] + [(n, c_int64) for n in (
+            "tokens", "batch", "heads", "kv_heads",
+            "q_stride_tok", "q_stride_head", "k_stride_tok", "k_stride_head", "v_stride_tok", "v_stride_head",
+            "qo_stride_tok", "qo_stride_head", "ko_stride_tok", "ko_stride_head",
+            "kc_stride_page", "kc_stride_tok", "kc_stride_head", "vc_stride_page", "vc_stride_tok", "vc_stride_head",
+            "table_stride", "rot_stride", "n_pages", "max_pages", "n_positions")] + [(n, c_int32) for n in (
+                "page_size", "head_dim", "rotary_dim", "interleaved", "dtype", "cache_dtype", "k_scale_n", "v_scale_n")]
+
+
+class AttentionDecodeArgs(Structure):
+    _fields_ = [(n, c_void_p) for n in (
+        "q", "k_cache", "v_cache", "o", "lse", "page_table", "seq_lens", "k_scale", "v_scale", "workspace")] + [
+            ("workspace_bytes", c_size_t)] + [(n, c_int64) for n in (
+                "batch", "heads", "kv_heads", "q_stride_b", "q_stride_head", "o_stride_b", "o_stride_head",
+                "kc_stride_page", "kc_stride_tok", "kc_stride_head", "vc_stride_page", "vc_stride_tok", "vc_stride_head",
+                "table_stride", "n_pages", "max_pages")] + [(n, c_int32) for n in (
+                    "page_size", "head_dim", "dtype", "cache_dtype", "k_scale_n", "v_scale_n")] + [
+                        ("sm_scale", c_float), ("reserved", c_int32)]
+
+
+class AttentionVarlenArgs(Structure):
+    _fields_ = [(n, c_void_p) for n in (
+        "q", "k", "v", "o", "lse", "cu_seqlens_q", "cu_seqlens_k", "page_table", "seq_lens", "workspace")] + [
+            ("workspace_bytes", c_size_t)] + [(n, c_int64) for n in (
+                "tokens_q", "tokens_k", "batch", "heads", "kv_heads",
+                "q_stride_tok", "q_stride_head", "o_stride_tok", "o_stride_head",
+                "k_stride_page", "k_stride_tok", "k_stride_head", "v_stride_page", "v_stride_tok", "v_stride_head",
+                "table_stride", "n_pages", "max_pages")] + [(n, c_int32) for n in (
+                    "page_size", "head_dim", "dtype", "causal")] + [("sm_scale", c_float), ("reserved", c_int32)]
+
+
 class TopkArgs(Structure):
     _fields_ = [
         ("x", c_void_p), ("y_vals", c_void_p), ("y_indx", c_void_p), ("bitmatrix", c_void_p),
@@ -214,7 +248,13 @@ def _declare(l: ctypes.CDLL) -> None:
     l.tb200_attention_bwd.argtypes = [POINTER(AttentionBwdArgs), c_void_p]
     l.tb200_attention_bwd_workspace_bytes.restype = c_size_t
     l.tb200_attention_bwd_workspace_bytes.argtypes = [POINTER(AttentionBwdArgs)]
-    for name, typ in (("tb200_topk", TopkArgs), ("tb200_bitmatrix_metadata", BitmatrixMetadataArgs),
+    l.tb200_attention_decode_workspace_bytes.restype = c_size_t
+    l.tb200_attention_decode_workspace_bytes.argtypes = [POINTER(AttentionDecodeArgs)]
+    l.tb200_attention_varlen_workspace_bytes.restype = c_size_t
+    l.tb200_attention_varlen_workspace_bytes.argtypes = [POINTER(AttentionVarlenArgs)]
+    for name, typ in (("tb200_kv_append", KvAppendArgs), ("tb200_attention_decode", AttentionDecodeArgs),
+                      ("tb200_attention_varlen_fwd", AttentionVarlenArgs),
+                      ("tb200_topk", TopkArgs), ("tb200_bitmatrix_metadata", BitmatrixMetadataArgs),
                       ("tb200_ragged_metadata", RaggedMetadataArgs), ("tb200_reduce_k", ReduceKArgs),
                       ("tb200_swiglu", SwigluArgs), ("tb200_moe_gemm", MoeGemmArgs),
                       ("tb200_remap_ragged_metadata", RemapRaggedMetadataArgs), ("tb200_ep_dispatch", EpDispatchArgs),
