@@ -1,7 +1,19 @@
 // Attention of one new token per sequence over a paged KV cache.
 //
-// One warp per (sequence, query head): lane l holds columns l * D/32 .. of the query, the accumulator and the key /
-// value row in flight; the score is a butterfly sum, the softmax is kept online (running maximum and sum in fp32).
+// The work is every (sequence, kv head, group of up to 8 NT query heads) times its KV tiles, laid out as one line of
+// tiles; each CTA takes an equal piece of the line, whatever the lengths are. A sequence's stretch that one CTA covers
+// alone is written out directly; the parts of one that is cut at CTA borders go to the workspace as (unnormalised
+// accumulator, maximum, sum) and a second small kernel joins them, in the order of the line (no atomics: equal inputs
+// give equal bits).
+//
+// Inside a CTA, a tile is 4 x KS keys: warp w takes keys w KS .. of every tile with a softmax of its own and the four are
+// merged through shared memory at the end of a stretch, so the loop has no block-wide barrier. Each warp keeps a ring of
+// steps in flight by 16-byte cp.async (keys behind the end and pages outside the pool are filled with zeros without an
+// access). The products run on the tensor cores with the keys as the long side: S^T [16 keys, 8 heads] = K Q^T and
+// O^T [16 columns, 8 heads] += V^T P^T by mma.m16n8k16, so a group of up to 8 heads fills the 8-wide side whatever its
+// size. tcgen05 has no use here: its 128-row tile would be filled by 8 heads, and the kernel is bound by reading K and V.
+// e4m3 pools are widened to float16 in registers (exact); queries are then brought to [1, 2) by a power of two per head
+// first, so that they fit. P is rounded to the type of V (float16 for e4m3), everything else is kept in 32 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <string.h>
@@ -12,73 +24,610 @@
 
 namespace tb200 {
 
+static constexpr int DEC_WARPS = 4;
+static constexpr float DEC_RESCALE_THRESHOLD = 8.0f;  // the accumulator is rescaled when a maximum grew by more than 2^8
+
+enum DecKind { DEC_BF16 = 0, DEC_F16 = 1, DEC_E4M3 = 2 };
+
+// One CTA's first stretch: the line positions [s, e) of the whole stretch, for the join.
+struct DecMeta {
+  int b, hg;
+  long long s, e;
+};
+
 struct DecodeParams {
   tb200_attention_decode_args a;
   float scale_log2;
+  int group, groups_per_kv, hgs;  // query heads per kv head; head groups per kv head; head groups in all
+  int max_len;
+  float* part_o;                  // [CTA][2][heads of a group][D]: a stretch cut at the CTA's start (0) or end (1)
+  float2* part_ml;                // [CTA][2][heads of a group]
+  DecMeta* meta;                  // [CTA]
+  long long* per;                 // tiles per CTA
 };
 
-template <int D, bool F16, bool C8>
-__global__ void __launch_bounds__(128) attention_decode_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int V = D / 32;
-  const tb200_attention_decode_args& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= a.batch * a.heads) return;
-  const int64_t b = row / a.heads, h = row % a.heads, kvh = h / (a.heads / a.kv_heads);
-  auto widen = [](uint16_t v) { return F16 ? __half2float(__ushort_as_half(v)) : __uint_as_float((uint32_t)v << 16); };
-  auto cached = [&](const void* pool, int64_t at) {
-    if (!C8) return widen(((const uint16_t*)pool)[at]);
-    uint32_t w;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(w) : "h"((uint16_t)((const uint8_t*)pool)[at]));
-    return __half2float(__ushort_as_half((uint16_t)w));
-  };
-  float q[V], o[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    q[i] = widen(((const uint16_t*)a.q)[b * a.q_stride_b + h * a.q_stride_head + lane * V + i]);
-    o[i] = 0.f;
-  }
-  float scale = p.scale_log2, v_scale = 1.f;
-  if (C8) {
-    scale *= a.k_scale[a.k_scale_n > 1 ? kvh : 0];
-    v_scale = a.v_scale[a.v_scale_n > 1 ? kvh : 0];
-  }
-  const int64_t len = min(max((int64_t)a.seq_lens[b], (int64_t)0), a.max_pages * a.page_size);
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < len; ++j) {
-    const int64_t page = a.page_table[b * a.table_stride + j / a.page_size], in_page = j % a.page_size;
-    const bool there = page >= 0 && page < a.n_pages;
-    const int64_t ka = page * a.kc_stride_page + in_page * a.kc_stride_tok + kvh * a.kc_stride_head + lane * V;
-    const int64_t va = page * a.vc_stride_page + in_page * a.vc_stride_tok + kvh * a.vc_stride_head + lane * V;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) s += there ? q[i] * cached(a.k_cache, ka + i) : 0.f;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= scale;
-    const float m_new = fmaxf(m, s), m_ref = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = fast_exp2(m - m_ref), e = fast_exp2(s - m_ref);
-    l = l * alpha + e;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = o[i] * alpha + (there ? e * cached(a.v_cache, va + i) : 0.f);
-    m = m_new;
-  }
-  const float inv = l > 0.f ? v_scale / l : 0.f;
-  uint16_t* out = (uint16_t*)a.o + b * a.o_stride_b + h * a.o_stride_head + lane * V;
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-    out[i] = F16 ? __half_as_ushort(__float2half_rn(o[i] * inv)) : __bfloat16_as_ushort(__float2bfloat16_rn(o[i] * inv));
-  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? m + log2f(l) : -INFINITY;
+template <int D, int KIND, int NT>
+struct DecCfg {
+  static constexpr int ESZ = KIND == DEC_E4M3 ? 1 : 2;
+  static constexpr int ROW = D * ESZ;                    // bytes of a K or V row
+  static constexpr int CH = ROW / 16;                    // 16-byte chunks of it
+  static constexpr int KS = ROW >= 256 ? 16 : 32;        // keys per warp step
+  static constexpr int TILE = DEC_WARPS * KS;
+  static constexpr int STAGE = 2 * KS * ROW;             // K then V
+  static constexpr int CTAS = D == 256 ? 1 : 2;          // per SM; together they keep up to 192 KB in flight
+  static constexpr int STAGES = 196608 / (CTAS * DEC_WARPS * STAGE);
+  static constexpr int NH = 8 * NT;
+  static constexpr int OPITCH = D + 4;                   // floats: the four lanes of a fragment row land in different banks
+  static constexpr int RING = DEC_WARPS * STAGES * STAGE;
+  static constexpr int OBUF = DEC_WARPS * 8 * OPITCH * 4;
+  static constexpr int SMEM = RING + OBUF + DEC_WARPS * NH * 8;
+};
+
+__device__ __forceinline__ void dec_cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void dec_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void dec_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t dec_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <bool BF>
+__device__ __forceinline__ void dec_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t dec_widen_e4m3(uint32_t two) {  // the low two bytes -> two halves
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  return r;
+}
+__device__ __forceinline__ float2 dec_unpack(uint32_t w, bool f16) {
+  return f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w))
+             : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+__device__ __forceinline__ int dec_len(const DecodeParams& p, int b) { return min(max(p.a.seq_lens[b], 0), p.max_len); }
+
+// Finished values of query head `h` of sequence `b`: columns c, c + 1.
+__device__ __forceinline__ void dec_store(const DecodeParams& p, int b, int h, int c, float x, float y) {
+  uint16_t* out = (uint16_t*)p.a.o + (long long)b * p.a.o_stride_b + (long long)h * p.a.o_stride_head + c;
+  *reinterpret_cast<uint32_t*>(out) = p.a.dtype == TB200_F16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+}
+
+template <int D, int KIND, int NT>
+__global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
+    attention_decode_kernel(const __grid_constant__ DecodeParams p) {
+  using C = DecCfg<D, KIND, NT>;
+  constexpr int KT = C::KS / 16, KSTEPS = D / 16, STAGES = C::STAGES, NH = C::NH;
+  constexpr bool BF = KIND == DEC_BF16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* obuf = reinterpret_cast<float*>(smem + C::RING);
+  float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);  // [warp][head]
+  long long* sh_sum = reinterpret_cast<long long*>(obuf);  // [warp]; the head of the kernel borrows the merge buffer
+  long long& sh_rem = sh_sum[DEC_WARPS];
+  int& sh_b = *reinterpret_cast<int*>(sh_sum + DEC_WARPS + 1);
+  const tb200_attention_decode_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int batch = (int)a.batch;
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // ---- this CTA's piece of the line
+  const int chunk = (batch + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32);
+  const int b_lo = min((int)threadIdx.x * chunk, batch), b_hi = min(b_lo + chunk, batch);
+  long long mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += (long long)((dec_len(p, b) + C::TILE - 1) / C::TILE) * p.hgs;
+  long long upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) sh_sum[warp] = upto;
+  if (threadIdx.x == 0) sh_b = batch;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < DEC_WARPS; ++w) {
+    if (w < warp) upto += sh_sum[w];
+    total += sh_sum[w];
+  }
+  const long long per = max((total + gridDim.x - 1) / gridDim.x, 1ll);
+  const long long first = per * blockIdx.x, last = min(first + per, total);
+  if (first < last && upto - mine <= first && first < upto) {
+    long long at = upto - mine;
+    for (int b = b_lo; b < b_hi; ++b) {
+      const long long w = (long long)((dec_len(p, b) + C::TILE - 1) / C::TILE) * p.hgs;
+      if (first < at + w) {
+        sh_b = b;
+        sh_rem = first - at;
+        break;
+      }
+      at += w;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.per = per;
+  // sequences without a key
+  for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+    if (dec_len(p, b) > 0) continue;
+    for (int i = threadIdx.x; i < (int)a.heads * (D / 2); i += blockDim.x) dec_store(p, b, i / (D / 2), i % (D / 2) * 2, 0.f, 0.f);
+    if (a.lse)
+      for (int h = threadIdx.x; h < (int)a.heads; h += blockDim.x) a.lse[(long long)b * a.heads + h] = -INFINITY;
+  }
+  if (first >= last) {
+    if (threadIdx.x == 0) p.meta[blockIdx.x].b = -1;
+    return;
+  }
+
+  // ---- positions on the line: one runs ahead for the loads, one for the products
+  struct At {
+    int b, hg, t, nt, len;
+  };
+  auto enter = [&](At& x, int b) {
+    x.b = b;
+    x.len = dec_len(p, b);
+    x.nt = (x.len + C::TILE - 1) / C::TILE;
+  };
+  auto advance = [&](At& x) {
+    if (++x.t < x.nt) return;
+    x.t = 0;
+    if (++x.hg < p.hgs) return;
+    x.hg = 0;
+    int b = x.b + 1;
+    while (b < batch && dec_len(p, b) == 0) ++b;
+    if (b < batch) enter(x, b);
+  };
+  At ld;
+  enter(ld, sh_b);
+  ld.hg = (int)(sh_rem / ld.nt);
+  ld.t = (int)(sh_rem - (long long)ld.hg * ld.nt);
+  At cur = ld;
+  __syncthreads();  // the merge buffer is free from here on
+  if (threadIdx.x == 0) p.meta[blockIdx.x] = DecMeta{cur.b, cur.hg, first - cur.t, first - cur.t + cur.nt};
+
+  const uint32_t ring = smem_u32(smem) + warp * STAGES * C::STAGE;
+  const bool page_steps = a.page_size % C::KS == 0;  // then a step's keys lie in one page
+  long long to_load = last - first;
+  // Rows of one step: lane r looks up row r's place (page_steps: all lanes the step's), a step ahead of its copies.
+  long long k_at = 0, v_at = 0;
+  int rows = 0;        // rows of the step that exist
+  bool there = false;  // this lane's row (page_steps: the step) has a page
+  auto look_up = [&]() {
+    const int key0 = ld.t * C::TILE + warp * C::KS;
+    rows = min(ld.len - key0, C::KS);
+    there = false;
+    const int r = page_steps ? 0 : lane % C::KS;
+    if (r < rows) {
+      const int key = key0 + r, slot = key / a.page_size, in_page = key - slot * a.page_size;
+      const long long page = a.page_table[ld.b * a.table_stride + slot];
+      there = page >= 0 && page < a.n_pages;
+      const int kvh = ld.hg / p.groups_per_kv;
+      k_at = there ? page * a.kc_stride_page + in_page * a.kc_stride_tok + kvh * a.kc_stride_head : 0;
+      v_at = there ? page * a.vc_stride_page + in_page * a.vc_stride_tok + kvh * a.vc_stride_head : 0;
+    }
+  };
+  auto issue = [&](int stage) {
+    constexpr int RPI = 32 / C::CH;  // rows per copy instruction of the warp
+    const int c = lane % C::CH;
+    const uint8_t *kp = (const uint8_t*)a.k_cache, *vp = (const uint8_t*)a.v_cache;
+#pragma unroll
+    for (int i = 0; i < C::KS / RPI; ++i) {
+      const int r = i * RPI + lane / C::CH;
+      long long ka = k_at, va = v_at;
+      bool ok = there;
+      if (page_steps) {
+        ka += r * a.kc_stride_tok;
+        va += r * a.vc_stride_tok;
+      } else {
+        ka = __shfl_sync(0xffffffffu, k_at, r);
+        va = __shfl_sync(0xffffffffu, v_at, r);
+        ok = __shfl_sync(0xffffffffu, (int)there, r) != 0;
+      }
+      ok = ok && r < rows;
+      const int sw = C::CH >= 8 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+      const uint32_t dst = ring + stage * C::STAGE + r * C::ROW + sw * 16;
+      dec_cp16(dst, kp + (ok ? ka * C::ESZ + c * 16 : 0), ok);
+      dec_cp16(dst + C::KS * C::ROW, vp + (ok ? va * C::ESZ + c * 16 : 0), ok);
+    }
+  };
+  auto load_next = [&](int stage) {
+    if (to_load > 0) {
+      issue(stage);
+      advance(ld);
+      if (--to_load > 0) look_up();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) load_next(s);
+
+  // ---- the loop
+  uint32_t qf[NT][KSTEPS][2];
+  float o[NT][KSTEPS][4], m[NT][2], l[NT][2], sc[NT][2];
+  bool fresh = true;
+  int stage = 0;
+  for (long long at = first; at < last; ++at) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();
+    load_next(stage == 0 ? STAGES - 1 : stage - 1);
+    const int kvh = cur.hg / p.groups_per_kv, head0 = kvh * p.group + cur.hg % p.groups_per_kv * NH;
+    const int heads = min(NH, (kvh + 1) * p.group - head0);
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int h = nt * 8 + lane / 4;
+        const uint16_t* row = (const uint16_t*)a.q + cur.b * a.q_stride_b + (head0 + h) * a.q_stride_head;
+        if (KIND != DEC_E4M3) {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(row + k * 16 + 2 * (lane & 3));
+            qf[nt][k][0] = h < heads ? w[0] : 0u;
+            qf[nt][k][1] = h < heads ? w[4] : 0u;
+          }
+          sc[nt][0] = sc[nt][1] = p.scale_log2;
+        } else {
+          // columns 4t .. 4t + 3 of each 16, the order in which ldmatrix hands out bytes
+          const bool f16 = a.dtype == TB200_F16;
+          float most = 0.f;
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            uint2 w = make_uint2(0u, 0u);
+            if (h < heads) w = *reinterpret_cast<const uint2*>(row + k * 16 + 4 * (lane & 3));
+            const float2 x = dec_unpack(w.x, f16), y = dec_unpack(w.y, f16);
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+            qf[nt][k][0] = w.x;
+            qf[nt][k][1] = w.y;
+          }
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const bool usual = most > 1e-30f && most < 1e30f;
+          const int e = usual ? (int)((__float_as_uint(most) >> 23) & 0xff) - 127 : 0;
+          const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            const float2 x = dec_unpack(qf[nt][k][0], f16), y = dec_unpack(qf[nt][k][1], f16);
+            qf[nt][k][0] = pack_f16x2(x.x * down, x.y * down);
+            qf[nt][k][1] = pack_f16x2(y.x * down, y.y * down);
+          }
+          const float ks = p.scale_log2 * a.k_scale[a.k_scale_n > 1 ? kvh : 0];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) sc[nt][j] = ks * __shfl_sync(0xffffffffu, up, 4 * (2 * (lane & 3) + j));
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          m[nt][j] = -INFINITY;
+          l[nt][j] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[nt][k][i] = 0.f;
+      }
+    }
+    const int key0 = cur.t * C::TILE + warp * C::KS;
+    if (key0 < cur.len) {
+      const uint32_t ks_base = ring + stage * C::STAGE, vs_base = ks_base + C::KS * C::ROW;
+      // ---- scores
+      float s[KT][NT][4];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[kt][nt][i] = 0.f;
+        const int r = kt * 16 + (lane & 15);
+        const uint32_t row_at = ks_base + r * C::ROW;
+        const int x = C::CH >= 8 ? r & 7 : (r >> 1) & 3;
+#pragma unroll
+        for (int c = 0; c < C::CH / 2; ++c) {  // 32 bytes of the rows at a time
+          uint32_t f[4];
+          dec_ldsm(row_at + (((2 * c + (lane >> 4)) ^ x) << 4), f);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (KIND != DEC_E4M3) {
+              dec_mma<BF>(s[kt][nt], f[0], f[1], f[2], f[3], qf[nt][c][0], qf[nt][c][1]);
+            } else {
+              dec_mma<false>(s[kt][nt], dec_widen_e4m3(f[0]), dec_widen_e4m3(f[1]), dec_widen_e4m3(f[0] >> 16),
+                             dec_widen_e4m3(f[1] >> 16), qf[nt][2 * c % KSTEPS][0], qf[nt][2 * c % KSTEPS][1]);
+              dec_mma<false>(s[kt][nt], dec_widen_e4m3(f[2]), dec_widen_e4m3(f[3]), dec_widen_e4m3(f[2] >> 16),
+                             dec_widen_e4m3(f[3] >> 16), qf[nt][(2 * c + 1) % KSTEPS][0], qf[nt][(2 * c + 1) % KSTEPS][1]);
+            }
+          }
+        }
+      }
+      // ---- softmax: rows are keys (lane / 4 and 8 more), columns heads (2 (lane % 4) and the next)
+      const bool ragged = key0 + C::KS > cur.len;
+      float mx[NT][2];
+      bool grew = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float t = -INFINITY;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float& v = s[kt][nt][2 * u + j];
+              v *= sc[nt][j];
+              if (ragged && key0 + kt * 16 + u * 8 + lane / 4 >= cur.len) v = -INFINITY;
+              t = fmaxf(t, v);
+            }
+          mx[nt][j] = t;
+          grew = grew || t > m[nt][j] + DEC_RESCALE_THRESHOLD;
+        }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float t = fmaxf(mx[nt][j], m[nt][j]);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, w));
+            const float alpha = m[nt][j] == -INFINITY ? 0.f : fast_exp2(m[nt][j] - t);
+            m[nt][j] = t;
+            l[nt][j] *= alpha;
+#pragma unroll
+            for (int k = 0; k < KSTEPS; ++k) {
+              o[nt][k][j] *= alpha;
+              o[nt][k][2 + j] *= alpha;
+            }
+          }
+      }
+      // ---- P^T, and O^T += V^T P^T
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float e0 = fast_exp2(s[kt][nt][2 * u] - r0), e1 = fast_exp2(s[kt][nt][2 * u + 1] - r1);
+            l[nt][0] += e0;
+            l[nt][1] += e1;
+            pb[nt][u] = dec_transpose(BF ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1));
+          }
+        }
+        const int r = kt * 16 + (KIND != DEC_E4M3 ? (lane & 7) + ((lane >> 4) & 1) * 8 : lane & 15);
+        const uint32_t row_at = vs_base + r * C::ROW;
+        const int x = C::CH >= 8 ? r & 7 : (r >> 1) & 3;
+        const int half = KIND != DEC_E4M3 ? (lane >> 3) & 1 : lane >> 4;
+#pragma unroll
+        for (int c = 0; c < C::CH / 2; ++c) {
+          uint32_t f[4];
+          dec_ldsm_t(row_at + (((2 * c + half) ^ x) << 4), f);
+          if (KIND != DEC_E4M3) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) dec_mma<BF>(o[nt][c], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+          } else {
+            // a register holds columns 2u, 2u + 1 of two keys: rows u and u + 8 of the fragment stand for these columns
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = __byte_perm(f[i], 0, 0x3120);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              dec_mma<false>(o[nt][2 * c % KSTEPS], dec_widen_e4m3(f[0]), dec_widen_e4m3(f[0] >> 16), dec_widen_e4m3(f[1]),
+                             dec_widen_e4m3(f[1] >> 16), pb[nt][0], pb[nt][1]);
+              dec_mma<false>(o[nt][(2 * c + 1) % KSTEPS], dec_widen_e4m3(f[2]), dec_widen_e4m3(f[2] >> 16),
+                             dec_widen_e4m3(f[3]), dec_widen_e4m3(f[3] >> 16), pb[nt][0], pb[nt][1]);
+            }
+          }
+        }
+      }
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+    // ---- end of a stretch: merge the four warps, write the result or the part
+    const bool ends = cur.t + 1 == cur.nt;
+    if (ends || at + 1 == last) {
+      const long long s0 = at - cur.t;  // where the stretch begins on the line
+      const bool whole = ends && s0 >= first;
+      const int slot = s0 >= first ? 1 : 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], w);
+          if (lane < 4) mlbuf[warp * NH + nt * 8 + 2 * lane + j] = make_float2(m[nt][j], l[nt][j]);
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int col = k * 16 + (KIND != DEC_E4M3 ? lane / 4 + 8 * u : 2 * (lane / 4) + u);
+              obuf[(warp * 8 + 2 * (lane & 3) + j) * C::OPITCH + col] = o[nt][k][2 * u + j];
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * (D / 2); i += DEC_WARPS * 32) {
+          const int h = i / (D / 2), col = i % (D / 2) * 2, hh = nt * 8 + h;
+          if (hh >= heads) break;
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, mlbuf[w * NH + hh].x);
+          float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+          for (int w = 0; w < DEC_WARPS; ++w) {
+            const float2 ml = mlbuf[w * NH + hh];
+            const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+            const float2 v = *reinterpret_cast<const float2*>(&obuf[(w * 8 + h) * C::OPITCH + col]);
+            sum += f * ml.y;
+            x += f * v.x;
+            y += f * v.y;
+          }
+          if (whole) {
+            float inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (KIND == DEC_E4M3) inv *= a.v_scale[a.v_scale_n > 1 ? kvh : 0];
+            dec_store(p, cur.b, head0 + hh, col, x * inv, y * inv);
+            if (a.lse && col == 0) a.lse[(long long)cur.b * a.heads + head0 + hh] = top + log2f(sum);
+          } else {
+            const long long part = ((long long)blockIdx.x * 2 + slot) * NH + hh;
+            *reinterpret_cast<float2*>(p.part_o + part * D + col) = make_float2(x, y);
+            if (col == 0) p.part_ml[part] = make_float2(top, sum);
+          }
+        }
+        __syncthreads();
+      }
+      fresh = true;
+    }
+    advance(cur);
+  }
+}
+
+// Joins the parts of the stretch that is cut at the start of CTA blockIdx.x's piece for the first time: the end of the
+// CTA before, then the beginning of every CTA that it reaches into. One block per query head of the group.
+template <int D, int NH>
+__global__ void __launch_bounds__(128) attention_decode_join_kernel(const __grid_constant__ DecodeParams p, int ctas, int e4m3) {
+  constexpr int COLS = D / 4, LANES = 128 / COLS;  // threads along a row, rows at a time
+  __shared__ float weight[1024];
+  __shared__ float red[4], red2[4];
+  __shared__ float4 acc[128];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, h = blockIdx.y;
+  const DecMeta me = p.meta[c];
+  const long long per = *p.per;
+  if (me.b < 0 || me.s >= per * c || me.s < per * (c - 1)) return;
+  const int kvh = me.hg / p.groups_per_kv, head = kvh * p.group + me.hg % p.groups_per_kv * NH + h;
+  if (head >= (kvh + 1) * p.group) return;
+  const int parts = 1 + (int)((me.e + per - 1) / per) - c;  // at most ctas, which is at most 1024
+  auto part_of = [&](int i) { return i == 0 ? ((long long)(c - 1) * 2 + 1) * NH + h : (long long)(c + i - 1) * 2 * NH + h; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += 128) top = fmaxf(top, p.part_ml[part_of(i)].x);
+#pragma unroll
+  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < parts; i += 128) {
+    const float2 ml = p.part_ml[part_of(i)];
+    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    weight[i] = f;
+    sum += f * ml.y;
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+  if (lane == 0) red2[warp] = sum;
+  __syncthreads();
+  sum = (red2[0] + red2[1]) + (red2[2] + red2[3]);
+  const int col = threadIdx.x % COLS, from = threadIdx.x / COLS;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = from; i < parts; i += LANES) {
+    const float f = weight[i];
+    const float4 v = reinterpret_cast<const float4*>(p.part_o + part_of(i) * D)[col];
+    x.x += f * v.x;
+    x.y += f * v.y;
+    x.z += f * v.z;
+    x.w += f * v.w;
+  }
+  acc[threadIdx.x] = x;
+  __syncthreads();
+  if (from == 0) {
+    for (int i = 1; i < LANES; ++i) {
+      const float4 v = acc[i * COLS + col];
+      x.x += v.x;
+      x.y += v.y;
+      x.z += v.z;
+      x.w += v.w;
+    }
+    float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (e4m3) inv *= p.a.v_scale[p.a.v_scale_n > 1 ? kvh : 0];
+    dec_store(p, me.b, head, col * 4, x.x * inv, x.y * inv);
+    dec_store(p, me.b, head, col * 4 + 2, x.z * inv, x.w * inv);
+    if (p.a.lse && col == 0) p.a.lse[(long long)me.b * p.a.heads + head] = top + log2f(sum);
+  }
+}
+
+// What a call will launch: heads per group, CTAs, and the workspace they need.
+struct DecPlan {
+  int nh, ctas;
+  size_t off_ml, off_meta, off_per, bytes;
+};
+// A group of 8 query heads fills the narrow side of the mma; 16 per group halve the reads of K and V for larger groups
+// (head dim 256 keeps 8: two accumulators of 256 columns do not fit the registers).
+static DecPlan dec_plan(const tb200_attention_decode_args* a, int sms) {
+  DecPlan d;
+  d.nh = a->heads / a->kv_heads > 8 && a->head_dim <= 128 ? 16 : 8;
+  d.ctas = sms * (a->head_dim == 256 ? 1 : 2);
+  const size_t parts = (size_t)d.ctas * 2 * d.nh;
+  d.off_ml = parts * a->head_dim * sizeof(float);
+  d.off_meta = d.off_ml + parts * sizeof(float2);
+  d.off_per = d.off_meta + (size_t)d.ctas * sizeof(DecMeta);
+  d.bytes = d.off_per + 16;
+  return d;
+}
+
+template <int D, int KIND, int NT>
+static int launch_decode(const DecodeParams& p, int ctas, cudaStream_t stream) {
+  using C = DecCfg<D, KIND, NT>;
+  static_assert(C::STAGES >= 3 && C::CTAS * (C::SMEM + 1024) <= 233472, "shared memory budget");
+  auto kfn = attention_decode_kernel<D, KIND, NT>;
+  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TB200_ERR_CUDA;
+  kfn<<<ctas, DEC_WARPS * 32, C::SMEM, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, C::NH);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_err(cudaLaunchKernelEx(&cfg, attention_decode_join_kernel<D, C::NH>, p, ctas, (int)(KIND == DEC_E4M3)));
+}
+
+template <int D, int KIND>
+static int launch_decode_heads(const DecodeParams& p, const DecPlan& plan, cudaStream_t stream) {
+  if constexpr (D <= 128) {
+    if (plan.nh == 16) return launch_decode<D, KIND, 2>(p, plan.ctas, stream);
+  }
+  return launch_decode<D, KIND, 1>(p, plan.ctas, stream);
+}
 template <int D>
-static int launch_decode(const DecodeParams& p, cudaStream_t stream) {
-  const bool f16 = p.a.dtype == TB200_F16, c8 = p.a.cache_dtype == TB200_E4M3;
-  auto kfn = f16 ? (c8 ? attention_decode_kernel<D, true, true> : attention_decode_kernel<D, true, false>)
-                 : (c8 ? attention_decode_kernel<D, false, true> : attention_decode_kernel<D, false, false>);
-  const int64_t rows = p.a.batch * p.a.heads;
-  kfn<<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(p);
-  return cuda_err(cudaGetLastError());
+static int launch_decode_kind(const DecodeParams& p, const DecPlan& plan, cudaStream_t stream) {
+  return p.a.cache_dtype == TB200_E4M3  ? launch_decode_heads<D, DEC_E4M3>(p, plan, stream)
+         : p.a.cache_dtype == TB200_F16 ? launch_decode_heads<D, DEC_F16>(p, plan, stream)
+                                        : launch_decode_heads<D, DEC_BF16>(p, plan, stream);
+}
+
+static int dec_check(const tb200_attention_decode_args* a) {
+  if (!a) return TB200_ERR_BAD_ARG;
+  if (a->batch < 0 || a->heads < 0 || a->kv_heads < 1 || a->heads % a->kv_heads || a->n_pages < 0 || a->max_pages < 0 ||
+      a->page_size < 1)
+    return TB200_ERR_BAD_ARG;
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return TB200_ERR_UNSUPPORTED;
+  if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
+  if (a->cache_dtype != TB200_E4M3 && a->cache_dtype != a->dtype) return TB200_ERR_UNSUPPORTED;
+  if (a->batch > INT32_MAX || a->heads > (1 << 16) || a->batch * a->heads > INT32_MAX || a->max_pages > INT32_MAX ||
+      a->max_pages * a->page_size > (1 << 30))
+    return TB200_ERR_UNSUPPORTED;
+  return TB200_OK;
 }
 
 }  // namespace tb200
@@ -87,17 +636,16 @@ using namespace tb200;
 
 static bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-extern "C" size_t tb200_attention_decode_workspace_bytes(const tb200_attention_decode_args*) { return 0; }
+extern "C" size_t tb200_attention_decode_workspace_bytes(const tb200_attention_decode_args* a) {
+  if (dec_check(a) != TB200_OK || a->batch == 0 || a->heads == 0) return 0;
+  const int sms = sm_count();
+  return sms > 0 ? dec_plan(a, sms).bytes : 0;
+}
 
 extern "C" int tb200_attention_decode(const tb200_attention_decode_args* a, void* stream_) {
-  if (!a) return TB200_ERR_BAD_ARG;
-  if (a->batch < 0 || a->heads < 0 || a->kv_heads < 1 || a->heads % a->kv_heads || a->n_pages < 0 || a->max_pages < 0 ||
-      a->page_size < 1)
-    return TB200_ERR_BAD_ARG;
-  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return TB200_ERR_UNSUPPORTED;
-  if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
+  const int rc = dec_check(a);
+  if (rc != TB200_OK) return rc;
   const bool c8 = a->cache_dtype == TB200_E4M3;
-  if (!c8 && a->cache_dtype != a->dtype) return TB200_ERR_UNSUPPORTED;
   if (c8 && ((a->k_scale_n != 1 && a->k_scale_n != a->kv_heads) || (a->v_scale_n != 1 && a->v_scale_n != a->kv_heads)))
     return TB200_ERR_BAD_ARG;
   if (!(a->sm_scale > 0.f)) return TB200_ERR_BAD_ARG;
@@ -109,18 +657,29 @@ extern "C" int tb200_attention_decode(const tb200_attention_decode_args* a, void
                            a->vc_stride_page, a->vc_stride_tok, a->vc_stride_head};
   for (int64_t s : pools)
     if (s % (c8 ? 16 : 8)) return TB200_ERR_BAD_ARG;
-  if (a->batch > INT32_MAX || a->heads > (1 << 16) || a->batch * a->heads > INT32_MAX || a->max_pages > INT32_MAX ||
-      a->max_pages * a->page_size > (1 << 30))
-    return TB200_ERR_UNSUPPORTED;
   if (a->batch == 0 || a->heads == 0) return TB200_OK;
   if (!a->q || !a->o || !a->seq_lens || (a->n_pages > 0 && (!a->k_cache || !a->v_cache)) ||
       (a->max_pages > 0 && !a->page_table) || (c8 && (!a->k_scale || !a->v_scale)))
     return TB200_ERR_BAD_ARG;
+  const int sms = sm_count();
+  if (sms <= 0) return TB200_ERR_CUDA;
+  const DecPlan plan = dec_plan(a, sms);
+  if (plan.ctas > 1024) return TB200_ERR_UNSUPPORTED;
+  if (!a->workspace || off16(a->workspace) || a->workspace_bytes < plan.bytes) return TB200_ERR_BAD_ARG;
   DecodeParams p;
   memset(&p, 0, sizeof(p));
   p.a = *a;
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p.group = (int)(a->heads / a->kv_heads);
+  p.groups_per_kv = (p.group + plan.nh - 1) / plan.nh;
+  p.hgs = p.groups_per_kv * (int)a->kv_heads;
+  p.max_len = (int)(a->max_pages * a->page_size);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + plan.off_ml);
+  p.meta = reinterpret_cast<DecMeta*>(ws + plan.off_meta);
+  p.per = reinterpret_cast<long long*>(ws + plan.off_per);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  return a->head_dim == 64 ? launch_decode<64>(p, stream)
-         : a->head_dim == 128 ? launch_decode<128>(p, stream) : launch_decode<256>(p, stream);
+  return a->head_dim == 64 ? launch_decode_kind<64>(p, plan, stream)
+         : a->head_dim == 128 ? launch_decode_kind<128>(p, plan, stream) : launch_decode_kind<256>(p, plan, stream);
 }
