@@ -40,95 +40,120 @@ _DT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _HEAD_DIMS = (64, 128, 256)
 
 
+# The checks below run on every call of a decode step, whose kernels take a few microseconds: each tensor's shape and strides
+# are read once, and what is rare (copies, dimensions of size one) has a function of its own.
 def _check_q(q, what):
+    """Device index, tokens, heads and head_dim of the query rows."""
     if not q.is_cuda:
         raise RuntimeError(f"triton_b200 {what} needs CUDA tensors (there is no CPU path)")
     assert q.dim() == 3, f"{what}: rows are [tokens, heads, head_dim]"
     if q.dtype not in _DT:
         raise NotImplementedError(f"{what}: dtype {q.dtype} (bfloat16 and float16 are implemented)")
-    if q.shape[2] not in _HEAD_DIMS:
-        raise NotImplementedError(f"{what}: head_dim {q.shape[2]} (64, 128 and 256 are implemented)")
+    n, h, d = q.shape
+    if d not in _HEAD_DIMS:
+        raise NotImplementedError(f"{what}: head_dim {d} (64, 128 and 256 are implemented)")
+    return q.get_device(), n, h, d
 
 
-def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_grad(what):
+    if torch.is_grad_enabled():
         raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad(), or train with attention()")
 
 
-def _strides(t):
-    """Token and head stride of ``[tokens, heads, d]`` rows; a dimension of size one has the stride it would have packed."""
-    n, h, d = t.shape
-    sh = t.stride(1) if h > 1 else d
-    return (t.stride(0) if n > 1 else max(sh * h, d)), sh
-
-
-def _rows_ok(t):
-    st, sh = _strides(t)
-    return t.stride(2) == 1 and st % 8 == 0 and sh % 8 == 0 and min(st, sh) >= t.shape[2] and t.data_ptr() % 16 == 0
+def _packed_strides(t):
+    """Strides of rows or of a pool whose dimensions of size one have the stride they would have if packed."""
+    shape, strides = t.shape, list(t.stride())
+    size = 1
+    for i in range(t.dim() - 1, -1, -1):
+        if shape[i] == 1:
+            strides[i] = size
+        size = max(size, strides[i] * shape[i])
+    return strides
 
 
 def _in_rows(t):
-    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+    """(rows, token stride, head stride): t itself where the kernels can address it, else a packed copy."""
+    n, h, d = t.shape
+    st, sh, sd = t.stride()
+    if sd != 1 or (st | sh) & 7 or st < d or sh < d or t.data_ptr() & 15:
+        st, sh, sd = _packed_strides(t)
+        if sd != 1 or (st | sh) & 7 or st < d or sh < d or t.data_ptr() & 15:
+            return t.clone(memory_format=torch.contiguous_format), h * d, d
+    return t, st, sh
 
 
 def _out_rows(out, like, name):
+    """(rows, token stride, head stride) of a result shaped like `like`."""
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        _, h, d = like.shape
+        return torch.empty_like(like, memory_format=torch.contiguous_format), h * d, d
     assert out.shape == like.shape and out.dtype == like.dtype and out.device == like.device, \
         f"{name} has the shape, dtype and device of its input"
-    assert _rows_ok(out), f"{name}: contiguous head_dim, strides that are multiples of 8 elements, 16-byte aligned"
-    return out
+    rows, st, sh = _in_rows(out)
+    assert rows is out, f"{name}: contiguous head_dim, strides that are multiples of 8 elements, 16-byte aligned"
+    return out, st, sh
 
 
-def _index(t, dev, name, n=None):
+def _index(t, idx, name, n=None):
     """A vector of int32 on the device of the data (n: its length)."""
     assert t.dtype == torch.int32 and t.dim() == 1 and (n is None or t.shape[0] == n), f"{name}: int32, one dimension, {n} entries"
-    assert t.device == dev, f"{name} is on {t.device}, the data on {dev}"
-    return t.contiguous()
+    assert t.get_device() == idx, f"{name} is on {t.device}, the data on cuda:{idx}"
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _pool(t, dtype, dev, name):
-    """Page, token and head stride of a ``[pages, page_size, kv_heads, d]`` pool."""
-    assert t.dim() == 4 and t.dtype == dtype and t.device == dev, f"{name}: [pages, page_size, kv_heads, head_dim] on {dev}"
-    n, s, h, d = t.shape
-    st = [t.stride(i) if t.shape[i] > 1 else s * h * d for i in range(3)]
-    step = 16 // t.element_size()
-    assert t.stride(3) == 1 and all(x % step == 0 and x >= d for x in st) and t.data_ptr() % 16 == 0, \
-        f"{name}: contiguous head_dim, strides that are multiples of 16 bytes, 16-byte aligned"
-    return st
+def _pool_strides(t, d, step, name):
+    """Page, token and head stride of a ``[pages, page_size, kv_heads, d]`` pool (`step`: elements in 16 bytes)."""
+    a, b, c, e = t.stride()
+    if e != 1 or (a | b | c) & (step - 1) or a < d or b < d or c < d or t.data_ptr() & 15:
+        a, b, c, e = _packed_strides(t)
+        assert e == 1 and not (a | b | c) & (step - 1) and min(a, b, c) >= d and not t.data_ptr() & 15, \
+            f"{name}: contiguous head_dim, strides that are multiples of 16 bytes, 16-byte aligned"
+    return a, b, c
 
 
-def _check_cache(q, k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, what):
-    dev = q.device
-    assert k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype
-    n_pages, page_size, kv_heads, d = k_cache.shape
-    fp8 = k_cache.dtype == torch.float8_e4m3fn
-    if not fp8 and k_cache.dtype != q.dtype:
-        raise NotImplementedError(f"{what}: a {k_cache.dtype} cache with {q.dtype} queries")
-    assert d == q.shape[2] and page_size > 0 and kv_heads > 0 and q.shape[1] % kv_heads == 0
-    kst, vst = _pool(k_cache, k_cache.dtype, dev, "k_cache"), _pool(v_cache, k_cache.dtype, dev, "v_cache")
-    assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == dev, "page_table: int32 [batch, max_pages]"
-    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+def _check_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, idx, heads, d, dtype, what):
+    """The cache as the kernels take it: sizes, strides, index tensors, scales and their counts."""
+    assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype, "caches: two equal pools"
+    assert k_cache.get_device() == idx and v_cache.get_device() == idx, f"{what}: the caches are not on the device of the rows"
+    n_pages, page_size, kv_heads, dim = k_cache.shape
+    cache_dtype = k_cache.dtype
+    fp8 = cache_dtype == torch.float8_e4m3fn
+    if not fp8 and cache_dtype != dtype:
+        raise NotImplementedError(f"{what}: a {cache_dtype} cache with {dtype} rows")
+    assert dim == d and page_size > 0 and kv_heads > 0 and heads % kv_heads == 0
+    kst = _pool_strides(k_cache, d, 16 if fp8 else 8, "k_cache")
+    vst = _pool_strides(v_cache, d, 16 if fp8 else 8, "v_cache")
+    assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.get_device() == idx, \
+        "page_table: int32 [batch, max_pages] on the device of the rows"
+    batch, max_pages = page_table.shape
+    table_stride, one = page_table.stride()
+    if one != 1 and max_pages > 1:
         page_table = page_table.contiguous()
-    seq_lens = _index(seq_lens, dev, "seq_lens", page_table.shape[0])
+        table_stride = max_pages
+    seq_lens = _index(seq_lens, idx, "seq_lens", batch)
+    kn = vn = 0
     if fp8:
         assert k_scale is not None and v_scale is not None, "a float8_e4m3fn cache needs k_scale and v_scale"
-        for s in (k_scale, v_scale):
-            assert s.dtype == torch.float32 and s.numel() in (1, kv_heads) and s.device == dev, "scales: float32, one or one per kv head"
+        kn, vn = k_scale.numel(), v_scale.numel()
+        for t, n in ((k_scale, kn), (v_scale, vn)):
+            assert t.dtype == torch.float32 and (n == 1 or n == kv_heads) and t.get_device() == idx, \
+                "scales: float32, one element or one per kv head"
         k_scale, v_scale = k_scale.contiguous(), v_scale.contiguous()
     else:
         assert k_scale is None and v_scale is None, "scales belong to a float8_e4m3fn cache"
-    return kst, vst, page_table, seq_lens, k_scale, v_scale
+    return (n_pages, page_size, kv_heads, kst, vst, page_table, batch, max_pages, table_stride, seq_lens, k_scale, v_scale, kn, vn,
+            _lib.E4M3 if fp8 else _DT[dtype])
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(name, args, dev):
-    with _lib.device_guard(dev):
-        rc = getattr(_lib.lib(), name)(ctypes.byref(args), ctypes.c_void_p(_lib.current_stream_ptr(dev)))
-    _lib.check(rc, name)
+def _call(fn, args, idx, name):
+    with _lib.device_guard(idx):
+        rc = fn(ctypes.byref(args), _lib.current_stream_ptr(idx))
+    if rc:
+        _lib.check(rc, name)
 
 
 def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, *, cos=None, sin=None,
@@ -149,67 +174,65 @@ def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=
     """
     what = "append_paged_kv"
     rows = k if q is None else q
-    _check_q(rows, what)
-    _no_grad(what, q, k, v)
-    dev, d = k.device, k.shape[2]
-    assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == rows.dtype and rows.device == v.device == dev
-    assert rows.shape[0] == k.shape[0] and rows.shape[2] == d and k_cache.shape[2] == k.shape[1]
-    kst, vst, page_table, seq_lens, k_scale, v_scale = _check_cache(rows, k_cache, v_cache, page_table, seq_lens, k_scale,
-                                                                    v_scale, what)
-    tokens, batch = k.shape[0], page_table.shape[0]
+    idx, tokens, heads, d = _check_q(rows, what)
+    if k.requires_grad or v.requires_grad or rows.requires_grad:
+        _refuse_grad(what)
+    dtype = rows.dtype
+    assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == dtype and k.get_device() == v.get_device() == idx
+    n, kv, dk = k.shape
+    assert n == tokens and dk == d
+    (n_pages, page_size, kv_heads, kst, vst, page_table, batch, max_pages, table_stride, seq_lens, k_scale, v_scale, kn, vn,
+     cache_dt) = _check_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, idx, heads, d, dtype, what)
+    assert kv == kv_heads, "k and v have the heads of the cache"
     if cu_seqlens is None:
         assert tokens == batch, "without cu_seqlens there is one row per sequence"
     else:
-        cu_seqlens = _index(cu_seqlens, dev, "cu_seqlens", batch + 1)
+        cu_seqlens = _index(cu_seqlens, idx, "cu_seqlens", batch + 1)
     assert (cos is None) == (sin is None)
-    positions = rotary = rot_stride = 0
+    positions = half = 0
     if cos is not None:
         assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
-        assert cos.device == sin.device == dev
+        assert cos.get_device() == sin.get_device() == idx
         cos, sin = cos.contiguous(), sin.contiguous()
-        positions, rotary, rot_stride = cos.shape[0], 2 * cos.shape[1], cos.shape[1]
-        assert 0 < rotary <= d and rotary % 16 == 0, "rotary_dim: a multiple of 16, at most head_dim"
-    ko = None if k_out is None else _out_rows(k_out, k, "k_out")
-    qo = None if q is None else _out_rows(q_out, q, "q_out")
-    q = None if q is None else _in_rows(q)
-    k, v = _in_rows(k), _in_rows(v)
+        positions, half = cos.shape
+        assert 0 < 2 * half <= d and half % 8 == 0, "rotary_dim: a multiple of 16, at most head_dim"
+    qo, qos, qoh = (None, 0, 0) if q is None else _out_rows(q_out, q, "q_out")
+    ko, kos, koh = (None, 0, 0) if k_out is None else _out_rows(k_out, k, "k_out")
+    q, qs, qh = (None, 0, 0) if q is None else _in_rows(q)
+    k, ks, kh = _in_rows(k)
+    v, vs, vh = _in_rows(v)
     args = _lib.KvAppendArgs(
         _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(qo), _ptr(ko), k_cache.data_ptr(), v_cache.data_ptr(),
         page_table.data_ptr(), seq_lens.data_ptr(), _ptr(cu_seqlens), _ptr(cos), _ptr(sin), _ptr(k_scale), _ptr(v_scale),
-        tokens, batch, 0 if q is None else q.shape[1], k.shape[1],
-        *(_strides(q) if q is not None else (0, 0)), *_strides(k), *_strides(v),
-        *(_strides(qo) if q is not None else (0, 0)), *(_strides(ko) if ko is not None else (0, 0)), *kst, *vst,
-        page_table.stride(0), rot_stride, k_cache.shape[0], page_table.shape[1], positions,
-        k_cache.shape[1], d, rotary, 1 if interleaved else 0, _DT[k.dtype],
-        _lib.E4M3 if k_scale is not None else _DT[k.dtype],
-        0 if k_scale is None else k_scale.numel(), 0 if v_scale is None else v_scale.numel())
-    _call("tb200_kv_append", args, dev)
+        tokens, batch, 0 if q is None else heads, kv_heads, qs, qh, ks, kh, vs, vh, qos, qoh, kos, koh, *kst, *vst,
+        table_stride, half, n_pages, max_pages, positions, page_size, d, 2 * half, 1 if interleaved else 0, _DT[dtype], cache_dt,
+        kn, vn)
+    _call(_lib.lib().tb200_kv_append, args, idx, "tb200_kv_append")
     return qo
 
 
 def _decode(q, k_cache, v_cache, page_table, seq_lens, sm_scale, k_scale, v_scale, out, with_lse):
     what = "attention_decode"
-    _check_q(q, what)
-    _no_grad(what, q)
-    dev = q.device
-    kst, vst, page_table, seq_lens, k_scale, v_scale = _check_cache(q, k_cache, v_cache, page_table, seq_lens, k_scale,
-                                                                    v_scale, what)
-    batch, heads, d = q.shape
-    assert page_table.shape[0] == batch, "one query row per sequence"
-    o = _out_rows(out, q, "out")
-    q = _in_rows(q)
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=dev) if with_lse else None
+    idx, n, heads, d = _check_q(q, what)
+    if q.requires_grad:
+        _refuse_grad(what)
+    dtype = q.dtype
+    (n_pages, page_size, kv_heads, kst, vst, page_table, batch, max_pages, table_stride, seq_lens, k_scale, v_scale, kn, vn,
+     cache_dt) = _check_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, idx, heads, d, dtype, what)
+    assert n == batch, "one query row per sequence"
+    o, os, oh = _out_rows(out, q, "out")
+    q, qs, qh = _in_rows(q)
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if with_lse else None
     args = _lib.AttentionDecodeArgs(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _ptr(lse), page_table.data_ptr(),
-        seq_lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), None, 0, batch, heads, k_cache.shape[2],
-        *_strides(q), *_strides(o), *kst, *vst, page_table.stride(0), k_cache.shape[0], page_table.shape[1],
-        k_cache.shape[1], d, _DT[q.dtype], _lib.E4M3 if k_scale is not None else _DT[q.dtype],
-        0 if k_scale is None else k_scale.numel(), 0 if v_scale is None else v_scale.numel(), float(sm_scale))
-    need = _lib.lib().tb200_attention_decode_workspace_bytes(ctypes.byref(args))
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _call("tb200_attention_decode", args, dev)
+        seq_lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), None, 0, batch, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
+        table_stride, n_pages, max_pages, page_size, d, _DT[dtype], cache_dt, kn, vn, float(sm_scale))
+    lib = _lib.lib()
+    with _lib.device_guard(idx):
+        need = lib.tb200_attention_decode_workspace_bytes(ctypes.byref(args))
+    ws = q.new_empty(need // 2 + 1)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _call(lib.tb200_attention_decode, args, idx, "tb200_attention_decode")
     return o, lse
 
 
@@ -224,38 +247,40 @@ def attention_decode_with_lse(q, k_cache, v_cache, page_table, seq_lens, sm_scal
     return _decode(q, k_cache, v_cache, page_table, seq_lens, sm_scale, k_scale, v_scale, out, True)
 
 
-def _varlen(what, q, k, v, kst, vst, cu_q, cu_k, page_table, seq_lens, n_pages, page_size, kv_heads, sm_scale, causal, out,
-            with_lse):
-    dev = q.device
-    tokens, heads, d = q.shape
-    o = _out_rows(out, q, "out")
-    q = _in_rows(q)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if with_lse else None
+def _varlen(what, q, k, v, kst, vst, cu_q, cu_k, page_table, seq_lens, tokens_k, table_stride, n_pages, max_pages, page_size,
+            kv_heads, sm_scale, causal, out, with_lse):
+    idx, tokens, heads, d = q.get_device(), *q.shape
+    o, os, oh = _out_rows(out, q, "out")
+    q, qs, qh = _in_rows(q)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if with_lse else None
     args = _lib.AttentionVarlenArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), cu_q.data_ptr(), _ptr(cu_k), _ptr(page_table),
-        _ptr(seq_lens), None, 0, tokens, 0 if page_size else k.shape[0], cu_q.shape[0] - 1, heads, kv_heads,
-        *_strides(q), *_strides(o), *kst, *vst, page_table.stride(0) if page_size else 0, n_pages,
-        page_table.shape[1] if page_size else 0, page_size, d, _DT[q.dtype], 1 if causal else 0, float(sm_scale))
-    need = _lib.lib().tb200_attention_varlen_workspace_bytes(ctypes.byref(args))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _ptr(seq_lens), None, 0, tokens, tokens_k, cu_q.shape[0] - 1, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
+        table_stride, n_pages, max_pages, page_size, d, _DT[q.dtype], 1 if causal else 0, float(sm_scale))
+    lib = _lib.lib()
+    with _lib.device_guard(idx):
+        need = lib.tb200_attention_varlen_workspace_bytes(ctypes.byref(args))
+    ws = q.new_empty(need // 2 + 1)
     args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _call("tb200_attention_varlen_fwd", args, dev)
+    _call(lib.tb200_attention_varlen_fwd, args, idx, "tb200_attention_varlen_fwd")
     return o, lse
 
 
 def _varlen_packed(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal, out, with_lse):
     what = "attention_varlen"
-    _check_q(q, what)
-    _no_grad(what, q, k, v)
-    dev = q.device
-    assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == q.dtype and k.device == v.device == dev
-    assert k.shape[2] == q.shape[2] and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0
-    cu_q = _index(cu_seqlens_q, dev, "cu_seqlens_q")
+    idx, _, heads, d = _check_q(q, what)
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _refuse_grad(what)
+    assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == q.dtype and k.get_device() == v.get_device() == idx
+    tokens_k, kv_heads, dk = k.shape
+    assert dk == d and kv_heads > 0 and heads % kv_heads == 0
+    cu_q = _index(cu_seqlens_q, idx, "cu_seqlens_q")
     assert cu_q.shape[0] >= 1
-    cu_k = cu_q if cu_seqlens_k is cu_seqlens_q else _index(cu_seqlens_k, dev, "cu_seqlens_k", cu_q.shape[0])
-    k, v = _in_rows(k), _in_rows(v)
-    return _varlen(what, q, k, v, (0, *_strides(k)), (0, *_strides(v)), cu_q, cu_k, None, None, 0, 0, k.shape[1], sm_scale,
-                   causal, out, with_lse)
+    cu_k = cu_q if cu_seqlens_k is cu_seqlens_q else _index(cu_seqlens_k, idx, "cu_seqlens_k", cu_q.shape[0])
+    k, *kst = _in_rows(k)
+    v, *vst = _in_rows(v)
+    return _varlen(what, q, k, v, (0, *kst), (0, *vst), cu_q, cu_k, None, None, tokens_k, 0, 0, 0, 0, kv_heads, sm_scale, causal,
+                   out, with_lse)
 
 
 def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal, out=None):
@@ -272,16 +297,18 @@ def attention_varlen_with_lse(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, cau
 
 def _varlen_over_pages(q, k_cache, v_cache, cu_seqlens_q, page_table, seq_lens, sm_scale, causal, out, with_lse):
     what = "attention_varlen_paged"
-    _check_q(q, what)
-    _no_grad(what, q)
+    idx, _, heads, d = _check_q(q, what)
+    if q.requires_grad:
+        _refuse_grad(what)
     if k_cache.dtype == torch.float8_e4m3fn:
         raise NotImplementedError(f"{what}: 8-bit caches are read by attention_decode only")
-    if k_cache.shape[1] % 8:
-        raise NotImplementedError(f"{what}: page_size {k_cache.shape[1]} (multiples of 8 are implemented)")
-    kst, vst, page_table, seq_lens, _, _ = _check_cache(q, k_cache, v_cache, page_table, seq_lens, None, None, what)
-    cu_q = _index(cu_seqlens_q, q.device, "cu_seqlens_q", page_table.shape[0] + 1)
-    return _varlen(what, q, k_cache, v_cache, kst, vst, cu_q, None, page_table, seq_lens, k_cache.shape[0], k_cache.shape[1],
-                   k_cache.shape[2], sm_scale, causal, out, with_lse)
+    n_pages, page_size, kv_heads, kst, vst, page_table, batch, max_pages, table_stride, seq_lens, *_ = _check_cache(
+        k_cache, v_cache, page_table, seq_lens, None, None, idx, heads, d, q.dtype, what)
+    if page_size % 8:
+        raise NotImplementedError(f"{what}: page_size {page_size} (multiples of 8 are implemented)")
+    cu_q = _index(cu_seqlens_q, idx, "cu_seqlens_q", batch + 1)
+    return _varlen(what, q, k_cache, v_cache, kst, vst, cu_q, None, page_table, seq_lens, 0, table_stride, n_pages, max_pages,
+                   page_size, kv_heads, sm_scale, causal, out, with_lse)
 
 
 def attention_varlen_paged(q, k_cache, v_cache, cu_seqlens_q, page_table, seq_lens, sm_scale, causal, out=None):
