@@ -1,17 +1,16 @@
 // Attention of one new token per sequence over a paged KV cache.
 //
-// The work is every (sequence, kv head, group of up to 8 NT query heads) times its KV tiles, laid out as one line of
-// tiles; each CTA takes an equal piece of the line, whatever the lengths are. A sequence's stretch that one CTA covers
-// alone is written out directly; the parts of one that is cut at CTA borders go to the workspace as (unnormalised
-// accumulator, maximum, sum) and a second small kernel joins them, in the order of the line (no atomics: equal inputs
-// give equal bits).
+// The work is every (sequence, kv head, group of up to 8 NT query heads) times its tiles of KS keys, laid out as one line of
+// tiles; each warp takes an equal piece of the line, whatever the lengths are, and runs on its own: a stretch (the tiles of one
+// sequence and head group) that lies in its piece is written out from its registers. Parts of stretches that are cut at
+// the borders of pieces are (unnormalised accumulator, maximum, sum); those inside a CTA are merged through shared memory at
+// the CTA's end, those between CTAs go to the workspace and a second small kernel joins them, in the order of the line (no
+// atomics: equal inputs give equal bits).
 //
-// Inside a CTA, a tile is 4 x KS keys: warp w takes keys w KS .. of every tile with a softmax of its own and the four are
-// merged through shared memory at the end of a stretch, so the loop has no block-wide barrier. Each warp keeps a ring of
-// steps in flight by 16-byte cp.async (keys behind the end and pages outside the pool are filled with zeros without an
-// access). The products run on the tensor cores with the keys as the long side: S^T [16 keys, 8 heads] = K Q^T and
-// O^T [16 columns, 8 heads] += V^T P^T by mma.m16n8k16, so a group of up to 8 heads fills the 8-wide side whatever its
-// size. tcgen05 has no use here: its 128-row tile would be filled by 8 heads, and the kernel is bound by reading K and V.
+// A warp keeps a ring of steps in flight by 16-byte cp.async (keys behind the end and pages outside the pool are filled with
+// zeros without an access). The products run on the tensor cores with the keys as the long side: S^T [16 keys, 8 heads] =
+// K Q^T and O^T [16 columns, 8 heads] += V^T P^T by mma.m16n8k16, so a group of up to 8 heads fills the 8-wide side whatever
+// its size. tcgen05 has no use here: its 128-row tile would be filled by 8 heads, and the kernel is bound by reading K and V.
 // e4m3 pools are widened to float16 in registers (exact); queries are then brought to [1, 2) by a power of two per head
 // first, so that they fit. P is rounded to the type of V (float16 for e4m3), everything else is kept in 32 bits.
 #include <cuda_bf16.h>
@@ -40,6 +39,9 @@ struct DecodeParams {
   float scale_log2;
   int group, groups_per_kv, hgs;  // query heads per kv head; head groups per kv head; head groups in all
   int max_len;
+  uint32_t page_mul, page_shift;  // n / page_size = umulhi(2 n, page_mul) >> page_shift for n < 2^30
+  long long k_page, k_tok, k_head, v_page, v_tok, v_head;  // strides of the pools in bytes
+  float* warp_o;                  // [CTA][parts of its warps][heads of a group][D]
   float* part_o;                  // [CTA][2][heads of a group][D]: a stretch cut at the CTA's start (0) or end (1)
   float2* part_ml;                // [CTA][2][heads of a group]
   DecMeta* meta;                  // [CTA]
@@ -51,16 +53,14 @@ struct DecCfg {
   static constexpr int ESZ = KIND == DEC_E4M3 ? 1 : 2;
   static constexpr int ROW = D * ESZ;                    // bytes of a K or V row
   static constexpr int CH = ROW / 16;                    // 16-byte chunks of it
-  static constexpr int KS = ROW >= 256 ? 16 : 32;        // keys per warp step
-  static constexpr int TILE = DEC_WARPS * KS;
+  static constexpr int KS = ROW >= 256 ? 16 : 32;        // keys per step
   static constexpr int STAGE = 2 * KS * ROW;             // K then V
   static constexpr int CTAS = D == 256 ? 1 : 2;          // per SM; together they keep up to 192 KB in flight
   static constexpr int STAGES = 196608 / (CTAS * DEC_WARPS * STAGE);
   static constexpr int NH = 8 * NT;
-  static constexpr int OPITCH = D + 4;                   // floats: the four lanes of a fragment row land in different banks
   static constexpr int RING = DEC_WARPS * STAGES * STAGE;
-  static constexpr int OBUF = DEC_WARPS * 8 * OPITCH * 4;
-  static constexpr int SMEM = RING + OBUF + DEC_WARPS * NH * 8;
+  static constexpr int PARTS = 2 * DEC_WARPS;            // of its warps' pieces, a cut stretch at each end
+  static constexpr int SMEM = RING + PARTS * NH * 8 + PARTS * 24;
 };
 
 __device__ __forceinline__ void dec_cp16(uint32_t dst, const void* src, bool there) {
@@ -109,34 +109,42 @@ __device__ __forceinline__ float2 dec_unpack(uint32_t w, bool f16) {
 
 __device__ __forceinline__ int dec_len(const DecodeParams& p, int b) { return min(max(p.a.seq_lens[b], 0), p.max_len); }
 
-// Finished values of query head `h` of sequence `b`: columns c, c + 1.
-__device__ __forceinline__ void dec_store(const DecodeParams& p, int b, int h, int c, float x, float y) {
-  uint16_t* out = (uint16_t*)p.a.o + (long long)b * p.a.o_stride_b + (long long)h * p.a.o_stride_head + c;
-  *reinterpret_cast<uint32_t*>(out) = p.a.dtype == TB200_F16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+__device__ __forceinline__ uint16_t* dec_out(const DecodeParams& p, int b, int h) {
+  return (uint16_t*)p.a.o + (long long)b * p.a.o_stride_b + (long long)h * p.a.o_stride_head;
 }
+__device__ __forceinline__ uint32_t dec_pack_out(const DecodeParams& p, float x, float y) {
+  return p.a.dtype == TB200_F16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+}
+
+// A stretch that a part in shared memory belongs to.
+struct DecPart {
+  long long s;  // where the stretch begins on the line; -1: no part
+  int b, hg, nt, pad;
+};
 
 template <int D, int KIND, int NT>
 __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     attention_decode_kernel(const __grid_constant__ DecodeParams p) {
   using C = DecCfg<D, KIND, NT>;
-  constexpr int KT = C::KS / 16, KSTEPS = D / 16, STAGES = C::STAGES, NH = C::NH;
+  constexpr int KT = C::KS / 16, KSTEPS = D / 16, STAGES = C::STAGES, NH = C::NH, RPI = 32 / C::CH;
   constexpr bool BF = KIND == DEC_BF16;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* obuf = reinterpret_cast<float*>(smem + C::RING);
-  float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);  // [warp][head]
-  long long* sh_sum = reinterpret_cast<long long*>(obuf);  // [warp]; the head of the kernel borrows the merge buffer
-  long long& sh_rem = sh_sum[DEC_WARPS];
-  int& sh_b = *reinterpret_cast<int*>(sh_sum + DEC_WARPS + 1);
+  float2* part_ml = reinterpret_cast<float2*>(smem + C::RING);                             // [part][head]
+  DecPart* parts = reinterpret_cast<DecPart*>(smem + C::RING + C::PARTS * NH * 8);          // [part]
+  // the head of the kernel borrows the ring
+  long long* sh_sum = reinterpret_cast<long long*>(smem);     // [warp]
+  long long* sh_rem = sh_sum + DEC_WARPS;                     // [warp]
+  int* sh_b = reinterpret_cast<int*>(sh_rem + DEC_WARPS);     // [warp]
   const tb200_attention_decode_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int batch = (int)a.batch;
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // ---- this CTA's piece of the line
+  // ---- this warp's piece of the line
   const int chunk = (batch + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32);
   const int b_lo = min((int)threadIdx.x * chunk, batch), b_hi = min(b_lo + chunk, batch);
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += (long long)((dec_len(p, b) + C::TILE - 1) / C::TILE) * p.hgs;
+  for (int b = b_lo; b < b_hi; ++b) mine += (long long)((dec_len(p, b) + C::KS - 1) / C::KS) * p.hgs;
   long long upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -144,7 +152,6 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     if (lane >= d) upto += o;
   }
   if (lane == 31) sh_sum[warp] = upto;
-  if (threadIdx.x == 0) sh_b = batch;
   __syncthreads();
   long long total = 0;
 #pragma unroll
@@ -152,348 +159,462 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     if (w < warp) upto += sh_sum[w];
     total += sh_sum[w];
   }
-  const long long per = max((total + gridDim.x - 1) / gridDim.x, 1ll);
-  const long long first = per * blockIdx.x, last = min(first + per, total);
-  if (first < last && upto - mine <= first && first < upto) {
-    long long at = upto - mine;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const long long w = (long long)((dec_len(p, b) + C::TILE - 1) / C::TILE) * p.hgs;
-      if (first < at + w) {
-        sh_b = b;
-        sh_rem = first - at;
-        break;
+  const long long per = max((total + gridDim.x * DEC_WARPS - 1) / (gridDim.x * DEC_WARPS), 1ll);  // tiles of a warp
+  const long long cta_first = per * DEC_WARPS * blockIdx.x, cta_last = min(cta_first + per * DEC_WARPS, total);
+#pragma unroll
+  for (int w = 0; w < DEC_WARPS; ++w) {
+    const long long target = cta_first + per * w;
+    if (target < upto && upto - mine <= target) {
+      long long at = upto - mine;
+      for (int b = b_lo; b < b_hi; ++b) {
+        const long long n = (long long)((dec_len(p, b) + C::KS - 1) / C::KS) * p.hgs;
+        if (target < at + n) {
+          sh_b[w] = b;
+          sh_rem[w] = target - at;
+          break;
+        }
+        at += n;
       }
-      at += w;
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.per = per;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.per = per * DEC_WARPS;
   // sequences without a key
   for (int b = blockIdx.x; b < batch; b += gridDim.x) {
     if (dec_len(p, b) > 0) continue;
-    for (int i = threadIdx.x; i < (int)a.heads * (D / 2); i += blockDim.x) dec_store(p, b, i / (D / 2), i % (D / 2) * 2, 0.f, 0.f);
+    for (int i = threadIdx.x; i < (int)a.heads * (D / 2); i += blockDim.x)
+      reinterpret_cast<uint32_t*>(dec_out(p, b, i / (D / 2)))[i % (D / 2)] = 0u;
     if (a.lse)
       for (int h = threadIdx.x; h < (int)a.heads; h += blockDim.x) a.lse[(long long)b * a.heads + h] = -INFINITY;
   }
-  if (first >= last) {
+  if (cta_first >= cta_last) {
     if (threadIdx.x == 0) p.meta[blockIdx.x].b = -1;
     return;
   }
+  const long long first = cta_first + per * warp, last = min(first + per, cta_last);
 
   // ---- positions on the line: one runs ahead for the loads, one for the products
   struct At {
     int b, hg, t, nt, len;
+    int next;  // the length of sequence b + 1, read ahead
   };
-  auto enter = [&](At& x, int b) {
+  auto enter = [&](At& x, int b, int len) {
     x.b = b;
-    x.len = dec_len(p, b);
-    x.nt = (x.len + C::TILE - 1) / C::TILE;
+    x.len = len;
+    x.nt = (len + C::KS - 1) / C::KS;
+    x.next = b + 1 < batch ? dec_len(p, b + 1) : 0;
   };
-  auto advance = [&](At& x) {
-    if (++x.t < x.nt) return;
+  auto next_stretch = [&](At& x) {
     x.t = 0;
     if (++x.hg < p.hgs) return;
     x.hg = 0;
-    int b = x.b + 1;
-    while (b < batch && dec_len(p, b) == 0) ++b;
-    if (b < batch) enter(x, b);
+    int b = x.b + 1, len = x.next;
+    while (len == 0 && b + 1 < batch) len = dec_len(p, ++b);
+    if (b < batch) enter(x, b, len);
   };
-  At ld;
-  enter(ld, sh_b);
-  ld.hg = (int)(sh_rem / ld.nt);
-  ld.t = (int)(sh_rem - (long long)ld.hg * ld.nt);
+  At ld = {};
+  const bool works = first < last;
+  if (works) {
+    const long long rem = sh_rem[warp];
+    enter(ld, sh_b[warp], dec_len(p, sh_b[warp]));
+    ld.hg = (int)(rem / ld.nt);
+    ld.t = (int)(rem - (long long)ld.hg * ld.nt);
+  }
   At cur = ld;
-  __syncthreads();  // the merge buffer is free from here on
   if (threadIdx.x == 0) p.meta[blockIdx.x] = DecMeta{cur.b, cur.hg, first - cur.t, first - cur.t + cur.nt};
+  __syncthreads();  // the ring is free from here on
+  if (lane < 2) parts[2 * warp + lane].s = -1;
 
   const uint32_t ring = smem_u32(smem) + warp * STAGES * C::STAGE;
   const bool page_steps = a.page_size % C::KS == 0;  // then a step's keys lie in one page
-  long long to_load = last - first;
-  // Rows of one step: lane r looks up row r's place (page_steps: all lanes the step's), a step ahead of its copies.
-  long long k_at = 0, v_at = 0;
-  int rows = 0;        // rows of the step that exist
-  bool there = false;  // this lane's row (page_steps: the step) has a page
+  const int row0 = lane / C::CH, col0 = lane % C::CH * 16;
+  // Places of a step's rows: lane r looks up row r (page_steps: all lanes the step's first row), a step ahead of its copies.
+  const uint8_t *k_at = nullptr, *v_at = nullptr;
+  long long k_kvh = 0, v_kvh = 0;  // byte offsets of the kv head
+  int rows = 0;                    // rows of the step that exist
+  bool there = false;              // this lane's row (page_steps: the step) has a page
+  auto enter_head = [&]() {
+    const int kvh = ld.hg / p.groups_per_kv;
+    k_kvh = kvh * p.k_head;
+    v_kvh = kvh * p.v_head;
+  };
   auto look_up = [&]() {
-    const int key0 = ld.t * C::TILE + warp * C::KS;
+    const int key0 = ld.t * C::KS;
     rows = min(ld.len - key0, C::KS);
     there = false;
     const int r = page_steps ? 0 : lane % C::KS;
     if (r < rows) {
-      const int key = key0 + r, slot = key / a.page_size, in_page = key - slot * a.page_size;
-      const long long page = a.page_table[ld.b * a.table_stride + slot];
-      there = page >= 0 && page < a.n_pages;
-      const int kvh = ld.hg / p.groups_per_kv;
-      k_at = there ? page * a.kc_stride_page + in_page * a.kc_stride_tok + kvh * a.kc_stride_head : 0;
-      v_at = there ? page * a.vc_stride_page + in_page * a.vc_stride_tok + kvh * a.vc_stride_head : 0;
+      const int key = key0 + r, slot = (int)(__umulhi((uint32_t)key * 2u, p.page_mul) >> p.page_shift);
+      const int in_page = key - slot * a.page_size;
+      const int page = a.page_table[ld.b * a.table_stride + slot];
+      there = page >= 0 && page < (int)a.n_pages;
+      k_at = (const uint8_t*)a.k_cache + page * p.k_page + in_page * p.k_tok + k_kvh;
+      v_at = (const uint8_t*)a.v_cache + page * p.v_page + in_page * p.v_tok + v_kvh;
     }
   };
+  // chunk c of row r goes to chunk c ^ (r % 8) (rows of 64 bytes: c ^ (r / 2 % 4)): eight rows at one column, which is
+  // what ldmatrix reads, lie in different banks
+  auto swizzle = [](int r) { return C::CH >= 8 ? (r & 7) << 4 : ((r >> 1) & 3) << 4; };
   auto issue = [&](int stage) {
-    constexpr int RPI = 32 / C::CH;  // rows per copy instruction of the warp
-    const int c = lane % C::CH;
-    const uint8_t *kp = (const uint8_t*)a.k_cache, *vp = (const uint8_t*)a.v_cache;
+    const uint32_t dst = ring + stage * C::STAGE + row0 * C::ROW;
+    if (page_steps && there && rows == C::KS) {
+      const uint8_t* kp = k_at + row0 * p.k_tok + col0;
+      const uint8_t* vp = v_at + row0 * p.v_tok + col0;
+      const long long k_step = RPI * p.k_tok, v_step = RPI * p.v_tok;
+#pragma unroll
+      for (int i = 0; i < C::KS / RPI; ++i) {
+        const uint32_t to = dst + i * RPI * C::ROW + (col0 ^ swizzle(i * RPI + row0));
+        dec_cp16(to, kp, true);
+        dec_cp16(to + C::KS * C::ROW, vp, true);
+        kp += k_step;
+        vp += v_step;
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < C::KS / RPI; ++i) {
-      const int r = i * RPI + lane / C::CH;
-      long long ka = k_at, va = v_at;
+      const int r = i * RPI + row0;
+      const uint8_t *kp, *vp;
       bool ok = there;
       if (page_steps) {
-        ka += r * a.kc_stride_tok;
-        va += r * a.vc_stride_tok;
+        kp = k_at + r * p.k_tok;
+        vp = v_at + r * p.v_tok;
       } else {
-        ka = __shfl_sync(0xffffffffu, k_at, r);
-        va = __shfl_sync(0xffffffffu, v_at, r);
+        kp = (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)k_at, r);
+        vp = (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)v_at, r);
         ok = __shfl_sync(0xffffffffu, (int)there, r) != 0;
       }
       ok = ok && r < rows;
-      const int sw = C::CH >= 8 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
-      const uint32_t dst = ring + stage * C::STAGE + r * C::ROW + sw * 16;
-      dec_cp16(dst, kp + (ok ? ka * C::ESZ + c * 16 : 0), ok);
-      dec_cp16(dst + C::KS * C::ROW, vp + (ok ? va * C::ESZ + c * 16 : 0), ok);
+      const uint32_t to = dst + i * RPI * C::ROW + (col0 ^ swizzle(r));
+      dec_cp16(to, ok ? kp + col0 : (const uint8_t*)a.k_cache, ok);
+      dec_cp16(to + C::KS * C::ROW, ok ? vp + col0 : (const uint8_t*)a.v_cache, ok);
     }
   };
+  long long to_load = last - first;
   auto load_next = [&](int stage) {
     if (to_load > 0) {
       issue(stage);
-      advance(ld);
-      if (--to_load > 0) look_up();
+      if (--to_load > 0) {
+        if (++ld.t == ld.nt) {
+          next_stretch(ld);
+          enter_head();
+        }
+        look_up();
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  look_up();
+
+  // ---- queries of the stretch ahead: the words as they are, and what they become
+  uint32_t qf[NT][KSTEPS][2];
+  int kvh = 0, head0 = 0, heads = 0;
+  auto load_q = [&](const At& x) {
+    kvh = x.hg / p.groups_per_kv;
+    head0 = kvh * p.group + (x.hg - kvh * p.groups_per_kv) * NH;
+    heads = min(NH, (kvh + 1) * p.group - head0);
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) load_next(s);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + lane / 4;
+      const uint16_t* row = (const uint16_t*)a.q + x.b * a.q_stride_b + (head0 + h) * a.q_stride_head;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        qf[nt][k][0] = qf[nt][k][1] = 0u;
+        if (h < heads) {
+          if (KIND != DEC_E4M3) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(row + k * 16 + 2 * (lane & 3));
+            qf[nt][k][0] = w[0];
+            qf[nt][k][1] = w[4];
+          } else {  // columns 4t .. 4t + 3 of each 16, the order in which ldmatrix hands out bytes
+            const uint2 w = *reinterpret_cast<const uint2*>(row + k * 16 + 4 * (lane & 3));
+            qf[nt][k][0] = w.x;
+            qf[nt][k][1] = w.y;
+          }
+        }
+      }
+    }
+  };
+  float o[NT][KSTEPS][4], m[NT][2], l[NT][2], sc[NT][2];
+  auto begin = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sc[nt][0] = sc[nt][1] = p.scale_log2;
+      if (KIND == DEC_E4M3) {
+        const bool f16 = a.dtype == TB200_F16;
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) {
+          const float2 x = dec_unpack(qf[nt][k][0], f16), y = dec_unpack(qf[nt][k][1], f16);
+          most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const bool usual = most > 1e-30f && most < 1e30f;
+        const int e = usual ? (int)((__float_as_uint(most) >> 23) & 0xff) - 127 : 0;
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) {
+          const float2 x = dec_unpack(qf[nt][k][0], f16), y = dec_unpack(qf[nt][k][1], f16);
+          qf[nt][k][0] = pack_f16x2(x.x * down, x.y * down);
+          qf[nt][k][1] = pack_f16x2(y.x * down, y.y * down);
+        }
+        const float ks = p.scale_log2 * a.k_scale[a.k_scale_n > 1 ? kvh : 0];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sc[nt][j] = ks * __shfl_sync(0xffffffffu, up, 4 * (2 * (lane & 3) + j));
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[nt][j] = -INFINITY;
+        l[nt][j] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][k][i] = 0.f;
+    }
+  };
+  if (works) {
+    load_q(cur);
+    enter_head();
+    look_up();
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) load_next(s);
+  }
 
   // ---- the loop
-  uint32_t qf[NT][KSTEPS][2];
-  float o[NT][KSTEPS][4], m[NT][2], l[NT][2], sc[NT][2];
   bool fresh = true;
   int stage = 0;
   for (long long at = first; at < last; ++at) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();
     load_next(stage == 0 ? STAGES - 1 : stage - 1);
-    const int kvh = cur.hg / p.groups_per_kv, head0 = kvh * p.group + cur.hg % p.groups_per_kv * NH;
-    const int heads = min(NH, (kvh + 1) * p.group - head0);
-    if (fresh) {
-      fresh = false;
+    if (fresh) begin();
+    fresh = false;
+    const int key0 = cur.t * C::KS;
+    const uint32_t ks_base = ring + stage * C::STAGE, vs_base = ks_base + C::KS * C::ROW;
+    // ---- scores
+    float s[KT][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int h = nt * 8 + lane / 4;
-        const uint16_t* row = (const uint16_t*)a.q + cur.b * a.q_stride_b + (head0 + h) * a.q_stride_head;
-        if (KIND != DEC_E4M3) {
+    for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(row + k * 16 + 2 * (lane & 3));
-            qf[nt][k][0] = h < heads ? w[0] : 0u;
-            qf[nt][k][1] = h < heads ? w[4] : 0u;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[kt][nt][i] = 0.f;
+      const int r = kt * 16 + (lane & 15);
+      const uint32_t row_at = ks_base + r * C::ROW;
+      const int x = swizzle(r);
+#pragma unroll
+      for (int c = 0; c < C::CH / 2; ++c) {  // 32 bytes of the rows at a time
+        uint32_t f[4];
+        dec_ldsm(row_at + (((2 * c + (lane >> 4)) << 4) ^ x), f);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (KIND != DEC_E4M3) {
+            dec_mma<BF>(s[kt][nt], f[0], f[1], f[2], f[3], qf[nt][c][0], qf[nt][c][1]);
+          } else {
+            dec_mma<false>(s[kt][nt], dec_widen_e4m3(f[0]), dec_widen_e4m3(f[1]), dec_widen_e4m3(f[0] >> 16),
+                           dec_widen_e4m3(f[1] >> 16), qf[nt][2 * c % KSTEPS][0], qf[nt][2 * c % KSTEPS][1]);
+            dec_mma<false>(s[kt][nt], dec_widen_e4m3(f[2]), dec_widen_e4m3(f[3]), dec_widen_e4m3(f[2] >> 16),
+                           dec_widen_e4m3(f[3] >> 16), qf[nt][(2 * c + 1) % KSTEPS][0], qf[nt][(2 * c + 1) % KSTEPS][1]);
           }
-          sc[nt][0] = sc[nt][1] = p.scale_log2;
-        } else {
-          // columns 4t .. 4t + 3 of each 16, the order in which ldmatrix hands out bytes
-          const bool f16 = a.dtype == TB200_F16;
-          float most = 0.f;
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
-            uint2 w = make_uint2(0u, 0u);
-            if (h < heads) w = *reinterpret_cast<const uint2*>(row + k * 16 + 4 * (lane & 3));
-            const float2 x = dec_unpack(w.x, f16), y = dec_unpack(w.y, f16);
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
-            qf[nt][k][0] = w.x;
-            qf[nt][k][1] = w.y;
-          }
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          const bool usual = most > 1e-30f && most < 1e30f;
-          const int e = usual ? (int)((__float_as_uint(most) >> 23) & 0xff) - 127 : 0;
-          const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
-            const float2 x = dec_unpack(qf[nt][k][0], f16), y = dec_unpack(qf[nt][k][1], f16);
-            qf[nt][k][0] = pack_f16x2(x.x * down, x.y * down);
-            qf[nt][k][1] = pack_f16x2(y.x * down, y.y * down);
-          }
-          const float ks = p.scale_log2 * a.k_scale[a.k_scale_n > 1 ? kvh : 0];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) sc[nt][j] = ks * __shfl_sync(0xffffffffu, up, 4 * (2 * (lane & 3) + j));
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          m[nt][j] = -INFINITY;
-          l[nt][j] = 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < KSTEPS; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[nt][k][i] = 0.f;
       }
     }
-    const int key0 = cur.t * C::TILE + warp * C::KS;
-    if (key0 < cur.len) {
-      const uint32_t ks_base = ring + stage * C::STAGE, vs_base = ks_base + C::KS * C::ROW;
-      // ---- scores
-      float s[KT][NT][4];
+    // ---- softmax: rows are keys (lane / 4 and 8 more), columns heads (2 (lane % 4) and the next)
+    const bool ragged = key0 + C::KS > cur.len;
+    float mx[NT][2];
+    bool grew = false;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < 2; ++j) {
+        float t = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[kt][nt][i] = 0.f;
-        const int r = kt * 16 + (lane & 15);
-        const uint32_t row_at = ks_base + r * C::ROW;
-        const int x = C::CH >= 8 ? r & 7 : (r >> 1) & 3;
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int c = 0; c < C::CH / 2; ++c) {  // 32 bytes of the rows at a time
-          uint32_t f[4];
-          dec_ldsm(row_at + (((2 * c + (lane >> 4)) ^ x) << 4), f);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (KIND != DEC_E4M3) {
-              dec_mma<BF>(s[kt][nt], f[0], f[1], f[2], f[3], qf[nt][c][0], qf[nt][c][1]);
-            } else {
-              dec_mma<false>(s[kt][nt], dec_widen_e4m3(f[0]), dec_widen_e4m3(f[1]), dec_widen_e4m3(f[0] >> 16),
-                             dec_widen_e4m3(f[1] >> 16), qf[nt][2 * c % KSTEPS][0], qf[nt][2 * c % KSTEPS][1]);
-              dec_mma<false>(s[kt][nt], dec_widen_e4m3(f[2]), dec_widen_e4m3(f[3]), dec_widen_e4m3(f[2] >> 16),
-                             dec_widen_e4m3(f[3] >> 16), qf[nt][(2 * c + 1) % KSTEPS][0], qf[nt][(2 * c + 1) % KSTEPS][1]);
-            }
+          for (int u = 0; u < 2; ++u) {
+            float& v = s[kt][nt][2 * u + j];
+            v *= sc[nt][j];
+            if (ragged && key0 + kt * 16 + u * 8 + lane / 4 >= cur.len) v = -INFINITY;
+            t = fmaxf(t, v);
           }
-        }
+        mx[nt][j] = t;
+        grew = grew || t > m[nt][j] + DEC_RESCALE_THRESHOLD;
       }
-      // ---- softmax: rows are keys (lane / 4 and 8 more), columns heads (2 (lane % 4) and the next)
-      const bool ragged = key0 + C::KS > cur.len;
-      float mx[NT][2];
-      bool grew = false;
+    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float t = -INFINITY;
+          float t = fmaxf(mx[nt][j], m[nt][j]);
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
+          for (int w = 4; w < 32; w <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, w));
+          const float alpha = m[nt][j] == -INFINITY ? 0.f : fast_exp2(m[nt][j] - t);
+          m[nt][j] = t;
+          l[nt][j] *= alpha;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float& v = s[kt][nt][2 * u + j];
-              v *= sc[nt][j];
-              if (ragged && key0 + kt * 16 + u * 8 + lane / 4 >= cur.len) v = -INFINITY;
-              t = fmaxf(t, v);
-            }
-          mx[nt][j] = t;
-          grew = grew || t > m[nt][j] + DEC_RESCALE_THRESHOLD;
-        }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float t = fmaxf(mx[nt][j], m[nt][j]);
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, w));
-            const float alpha = m[nt][j] == -INFINITY ? 0.f : fast_exp2(m[nt][j] - t);
-            m[nt][j] = t;
-            l[nt][j] *= alpha;
-#pragma unroll
-            for (int k = 0; k < KSTEPS; ++k) {
-              o[nt][k][j] *= alpha;
-              o[nt][k][2 + j] *= alpha;
-            }
+          for (int k = 0; k < KSTEPS; ++k) {
+            o[nt][k][j] *= alpha;
+            o[nt][k][2 + j] *= alpha;
           }
+        }
+    }
+    // ---- P^T, and O^T += V^T P^T
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float e0 = fast_exp2(s[kt][nt][2 * u] - r0), e1 = fast_exp2(s[kt][nt][2 * u + 1] - r1);
+          l[nt][0] += e0;
+          l[nt][1] += e1;
+          pb[nt][u] = dec_transpose(BF ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1));
+        }
       }
-      // ---- P^T, and O^T += V^T P^T
+      const int r = kt * 16 + (KIND != DEC_E4M3 ? (lane & 7) + ((lane >> 4) & 1) * 8 : lane & 15);
+      const uint32_t row_at = vs_base + r * C::ROW;
+      const int x = swizzle(r);
+      const int half = KIND != DEC_E4M3 ? (lane >> 3) & 1 : lane >> 4;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        uint32_t pb[NT][2];
+      for (int c = 0; c < C::CH / 2; ++c) {
+        uint32_t f[4];
+        dec_ldsm_t(row_at + (((2 * c + half) << 4) ^ x), f);
+        if (KIND != DEC_E4M3) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+          for (int nt = 0; nt < NT; ++nt) dec_mma<BF>(o[nt][c], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+        } else {
+          // a register holds columns 2u, 2u + 1 of two keys: rows u and u + 8 of the fragment stand for these columns
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float e0 = fast_exp2(s[kt][nt][2 * u] - r0), e1 = fast_exp2(s[kt][nt][2 * u + 1] - r1);
-            l[nt][0] += e0;
-            l[nt][1] += e1;
-            pb[nt][u] = dec_transpose(BF ? pack_bf16x2(e0, e1) : pack_f16x2(e0, e1));
-          }
-        }
-        const int r = kt * 16 + (KIND != DEC_E4M3 ? (lane & 7) + ((lane >> 4) & 1) * 8 : lane & 15);
-        const uint32_t row_at = vs_base + r * C::ROW;
-        const int x = C::CH >= 8 ? r & 7 : (r >> 1) & 3;
-        const int half = KIND != DEC_E4M3 ? (lane >> 3) & 1 : lane >> 4;
+          for (int i = 0; i < 4; ++i) f[i] = __byte_perm(f[i], 0, 0x3120);
 #pragma unroll
-        for (int c = 0; c < C::CH / 2; ++c) {
-          uint32_t f[4];
-          dec_ldsm_t(row_at + (((2 * c + half) ^ x) << 4), f);
-          if (KIND != DEC_E4M3) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) dec_mma<BF>(o[nt][c], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
-          } else {
-            // a register holds columns 2u, 2u + 1 of two keys: rows u and u + 8 of the fragment stand for these columns
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = __byte_perm(f[i], 0, 0x3120);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              dec_mma<false>(o[nt][2 * c % KSTEPS], dec_widen_e4m3(f[0]), dec_widen_e4m3(f[0] >> 16), dec_widen_e4m3(f[1]),
-                             dec_widen_e4m3(f[1] >> 16), pb[nt][0], pb[nt][1]);
-              dec_mma<false>(o[nt][(2 * c + 1) % KSTEPS], dec_widen_e4m3(f[2]), dec_widen_e4m3(f[2] >> 16),
-                             dec_widen_e4m3(f[3]), dec_widen_e4m3(f[3] >> 16), pb[nt][0], pb[nt][1]);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            dec_mma<false>(o[nt][2 * c % KSTEPS], dec_widen_e4m3(f[0]), dec_widen_e4m3(f[0] >> 16), dec_widen_e4m3(f[1]),
+                           dec_widen_e4m3(f[1] >> 16), pb[nt][0], pb[nt][1]);
+            dec_mma<false>(o[nt][(2 * c + 1) % KSTEPS], dec_widen_e4m3(f[2]), dec_widen_e4m3(f[2] >> 16),
+                           dec_widen_e4m3(f[3]), dec_widen_e4m3(f[3] >> 16), pb[nt][0], pb[nt][1]);
           }
         }
       }
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
+    if (++cur.t < cur.nt && at + 1 < last) continue;
 
-    // ---- end of a stretch: merge the four warps, write the result or the part
-    const bool ends = cur.t + 1 == cur.nt;
-    if (ends || at + 1 == last) {
-      const long long s0 = at - cur.t;  // where the stretch begins on the line
-      const bool whole = ends && s0 >= first;
-      const int slot = s0 >= first ? 1 : 0;
+    // ---- end of a stretch or of the piece
+    const long long s0 = at + 1 - cur.t;  // where the stretch begins on the line
+    const int b = cur.b, out_head = head0, out_heads = heads, out_kvh = kvh;
+    const bool whole = cur.t == cur.nt && s0 >= first;
+    const int done_hg = cur.hg, done_nt = cur.nt;
+    if (at + 1 < last) {
+      next_stretch(cur);
+      load_q(cur);  // under what follows
+    }
+    fresh = true;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], w);
+    if (whole) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        float inv[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+          inv[j] = l[nt][j] == 0.f ? 0.f : 1.f / l[nt][j];
+          if (KIND == DEC_E4M3) inv[j] *= a.v_scale[a.v_scale_n > 1 ? out_kvh : 0];
+          const int h = nt * 8 + 2 * lane + j;
+          if (a.lse && lane < 4 && h < out_heads)
+            a.lse[(long long)b * a.heads + out_head + h] = m[nt][j] + log2f(l[nt][j]);
+        }
+        const int h = nt * 8 + lane / 4;  // after the transposition: heads are rows
+        uint16_t* out = dec_out(p, b, out_head + h);
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], w);
-          if (lane < 4) mlbuf[warp * NH + nt * 8 + 2 * lane + j] = make_float2(m[nt][j], l[nt][j]);
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int col = k * 16 + (KIND != DEC_E4M3 ? lane / 4 + 8 * u : 2 * (lane / 4) + u);
-              obuf[(warp * 8 + 2 * (lane & 3) + j) * C::OPITCH + col] = o[nt][k][2 * u + j];
+        for (int k = 0; k < KSTEPS; ++k) {
+          uint32_t x = dec_transpose(dec_pack_out(p, o[nt][k][0] * inv[0], o[nt][k][1] * inv[1]));
+          uint32_t y = dec_transpose(dec_pack_out(p, o[nt][k][2] * inv[0], o[nt][k][3] * inv[1]));
+          if (h < out_heads) {
+            if (KIND != DEC_E4M3) {
+              *reinterpret_cast<uint32_t*>(out + k * 16 + 2 * (lane & 3)) = x;
+              *reinterpret_cast<uint32_t*>(out + k * 16 + 8 + 2 * (lane & 3)) = y;
+            } else {
+              *reinterpret_cast<uint2*>(out + k * 16 + 4 * (lane & 3)) =
+                  make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
             }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 8 * (D / 2); i += DEC_WARPS * 32) {
-          const int h = i / (D / 2), col = i % (D / 2) * 2, hh = nt * 8 + h;
-          if (hh >= heads) break;
-          float top = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, mlbuf[w * NH + hh].x);
-          float sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-          for (int w = 0; w < DEC_WARPS; ++w) {
-            const float2 ml = mlbuf[w * NH + hh];
-            const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-            const float2 v = *reinterpret_cast<const float2*>(&obuf[(w * 8 + h) * C::OPITCH + col]);
-            sum += f * ml.y;
-            x += f * v.x;
-            y += f * v.y;
-          }
-          if (whole) {
-            float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (KIND == DEC_E4M3) inv *= a.v_scale[a.v_scale_n > 1 ? kvh : 0];
-            dec_store(p, cur.b, head0 + hh, col, x * inv, y * inv);
-            if (a.lse && col == 0) a.lse[(long long)cur.b * a.heads + head0 + hh] = top + log2f(sum);
-          } else {
-            const long long part = ((long long)blockIdx.x * 2 + slot) * NH + hh;
-            *reinterpret_cast<float2*>(p.part_o + part * D + col) = make_float2(x, y);
-            if (col == 0) p.part_ml[part] = make_float2(top, sum);
           }
         }
-        __syncthreads();
       }
-      fresh = true;
+    } else {
+      // cut at the piece's start (part 2 w) or, begun here, at its end (part 2 w + 1)
+      const int part = 2 * warp + (s0 >= first ? 1 : 0);
+      if (lane == 0) parts[part] = DecPart{s0, b, done_hg, done_nt, 0};
+      float* dst = p.warp_o + ((long long)blockIdx.x * C::PARTS + part) * NH * D;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (lane < 4) part_ml[part * NH + nt * 8 + 2 * lane + j] = make_float2(m[nt][j], l[nt][j]);
+          float* row = dst + (nt * 8 + 2 * (lane & 3) + j) * D;
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            if (KIND != DEC_E4M3) {
+              row[k * 16 + lane / 4] = o[nt][k][j];
+              row[k * 16 + 8 + lane / 4] = o[nt][k][2 + j];
+            } else {
+              *reinterpret_cast<float2*>(row + k * 16 + lane / 4 * 2) = make_float2(o[nt][k][j], o[nt][k][2 + j]);
+            }
+          }
+        }
     }
-    advance(cur);
+  }
+
+  // ---- merge the parts of this CTA, stretch by stretch (they lie in the order of the line)
+  __syncthreads();
+  for (int i = 0; i < C::PARTS;) {
+    const DecPart me = parts[i];
+    if (me.s < 0) {
+      ++i;
+      continue;
+    }
+    int n = 1;  // parts i .. i + n - 1, without the empty ones, belong to this stretch
+    while (i + n < C::PARTS && (parts[i + n].s < 0 || parts[i + n].s == me.s)) ++n;
+    const bool whole = me.s >= cta_first && me.s + me.nt <= cta_last;
+    const int slot = me.s >= cta_first ? 1 : 0;
+    const int of_kv = me.hg / p.groups_per_kv, from = of_kv * p.group + (me.hg - of_kv * p.groups_per_kv) * NH;
+    const int n_heads = min(NH, (of_kv + 1) * p.group - from);
+    for (int e = threadIdx.x; e < n_heads * (D / 4); e += DEC_WARPS * 32) {
+      const int h = e / (D / 4), col = e % (D / 4) * 4;
+      float top = -INFINITY, sum = 0.f;
+      for (int q = i; q < i + n; ++q)
+        if (parts[q].s >= 0) top = fmaxf(top, part_ml[q * NH + h].x);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = i; q < i + n; ++q) {
+        if (parts[q].s < 0) continue;
+        const float2 ml = part_ml[q * NH + h];
+        const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+        const float4 v =
+            *reinterpret_cast<const float4*>(p.warp_o + (((long long)blockIdx.x * C::PARTS + q) * NH + h) * D + col);
+        sum += f * ml.y;
+        x.x += f * v.x;
+        x.y += f * v.y;
+        x.z += f * v.z;
+        x.w += f * v.w;
+      }
+      if (whole) {
+        float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (KIND == DEC_E4M3) inv *= a.v_scale[a.v_scale_n > 1 ? of_kv : 0];
+        *reinterpret_cast<uint2*>(dec_out(p, me.b, from + h) + col) =
+            make_uint2(dec_pack_out(p, x.x * inv, x.y * inv), dec_pack_out(p, x.z * inv, x.w * inv));
+        if (a.lse && col == 0) a.lse[(long long)me.b * a.heads + from + h] = top + log2f(sum);
+      } else {
+        const long long part = ((long long)blockIdx.x * 2 + slot) * NH + h;
+        *reinterpret_cast<float4*>(p.part_o + part * D + col) = x;
+        if (col == 0) p.part_ml[part] = make_float2(top, sum);
+      }
+    }
+    i += n;
   }
 }
 
@@ -557,8 +678,8 @@ __global__ void __launch_bounds__(128) attention_decode_join_kernel(const __grid
     }
     float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (e4m3) inv *= p.a.v_scale[p.a.v_scale_n > 1 ? kvh : 0];
-    dec_store(p, me.b, head, col * 4, x.x * inv, x.y * inv);
-    dec_store(p, me.b, head, col * 4 + 2, x.z * inv, x.w * inv);
+    *reinterpret_cast<uint2*>(dec_out(p, me.b, head) + col * 4) =
+        make_uint2(dec_pack_out(p, x.x * inv, x.y * inv), dec_pack_out(p, x.z * inv, x.w * inv));
     if (p.a.lse && col == 0) p.a.lse[(long long)me.b * p.a.heads + head] = top + log2f(sum);
   }
 }
@@ -566,7 +687,7 @@ __global__ void __launch_bounds__(128) attention_decode_join_kernel(const __grid
 // What a call will launch: heads per group, CTAs, and the workspace they need.
 struct DecPlan {
   int nh, ctas;
-  size_t off_ml, off_meta, off_per, bytes;
+  size_t off_warp, off_ml, off_meta, off_per, bytes;
 };
 // A group of 8 query heads fills the narrow side of the mma; 16 per group halve the reads of K and V for larger groups
 // (head dim 256 keeps 8: two accumulators of 256 columns do not fit the registers).
@@ -575,7 +696,8 @@ static DecPlan dec_plan(const tb200_attention_decode_args* a, int sms) {
   d.nh = a->heads / a->kv_heads > 8 && a->head_dim <= 128 ? 16 : 8;
   d.ctas = sms * (a->head_dim == 256 ? 1 : 2);
   const size_t parts = (size_t)d.ctas * 2 * d.nh;
-  d.off_ml = parts * a->head_dim * sizeof(float);
+  d.off_warp = parts * a->head_dim * sizeof(float);
+  d.off_ml = d.off_warp + parts * DEC_WARPS * a->head_dim * sizeof(float);
   d.off_meta = d.off_ml + parts * sizeof(float2);
   d.off_per = d.off_meta + (size_t)d.ctas * sizeof(DecMeta);
   d.bytes = d.off_per + 16;
@@ -625,6 +747,7 @@ static int dec_check(const tb200_attention_decode_args* a) {
   if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
   if (a->cache_dtype != TB200_E4M3 && a->cache_dtype != a->dtype) return TB200_ERR_UNSUPPORTED;
   if (a->batch > INT32_MAX || a->heads > (1 << 16) || a->batch * a->heads > INT32_MAX || a->max_pages > INT32_MAX ||
+      a->n_pages > INT32_MAX ||
       a->max_pages * a->page_size > (1 << 30))
     return TB200_ERR_UNSUPPORTED;
   return TB200_OK;
@@ -674,8 +797,18 @@ extern "C" int tb200_attention_decode(const tb200_attention_decode_args* a, void
   p.groups_per_kv = (p.group + plan.nh - 1) / plan.nh;
   p.hgs = p.groups_per_kv * (int)a->kv_heads;
   p.max_len = (int)(a->max_pages * a->page_size);
+  while ((1ll << p.page_shift) < a->page_size) ++p.page_shift;
+  p.page_mul = (uint32_t)((1ull << (31 + p.page_shift)) / (uint64_t)a->page_size + 1);
+  const int64_t size = c8 ? 1 : 2;
+  p.k_page = a->kc_stride_page * size;
+  p.k_tok = a->kc_stride_tok * size;
+  p.k_head = a->kc_stride_head * size;
+  p.v_page = a->vc_stride_page * size;
+  p.v_tok = a->vc_stride_tok * size;
+  p.v_head = a->vc_stride_head * size;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(ws);
+  p.warp_o = reinterpret_cast<float*>(ws + plan.off_warp);
   p.part_ml = reinterpret_cast<float2*>(ws + plan.off_ml);
   p.meta = reinterpret_cast<DecMeta*>(ws + plan.off_meta);
   p.per = reinterpret_cast<long long*>(ws + plan.off_per);
