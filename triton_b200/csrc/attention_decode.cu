@@ -30,8 +30,7 @@ enum DecKind { DEC_BF16 = 0, DEC_F16 = 1, DEC_E4M3 = 2 };
 
 // One CTA's first stretch: the line positions [s, e) of the whole stretch, for the join.
 struct DecMeta {
-  int b, hg;
-  long long s, e;
+  int b, hg, s, e;
 };
 
 struct DecodeParams {
@@ -41,11 +40,11 @@ struct DecodeParams {
   int max_len;
   uint32_t page_mul, page_shift;  // n / page_size = umulhi(2 n, page_mul) >> page_shift for n < 2^30
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;  // strides of the pools in bytes
-  float* warp_o;                  // [CTA][parts of its warps][heads of a group][D]
+  float* warp_o;                  // [CTA][warp][heads of a group][D]: parts cut at the start of a warp's piece
   float* part_o;                  // [CTA][2][heads of a group][D]: a stretch cut at the CTA's start (0) or end (1)
   float2* part_ml;                // [CTA][2][heads of a group]
   DecMeta* meta;                  // [CTA]
-  long long* per;                 // tiles per CTA
+  int* per;                       // tiles per CTA
 };
 
 template <int D, int KIND, int NT>
@@ -60,7 +59,14 @@ struct DecCfg {
   static constexpr int NH = 8 * NT;
   static constexpr int RING = DEC_WARPS * STAGES * STAGE;
   static constexpr int PARTS = 2 * DEC_WARPS;            // of its warps' pieces, a cut stretch at each end
-  static constexpr int SMEM = RING + PARTS * NH * 8 + PARTS * 24;
+  static constexpr int HEAD = NH * D * 4;                // bytes of a part's accumulator
+  static constexpr int LIMIT = 233472 / CTAS - 1024;
+  // A part that is cut at a piece's end takes the place of the warp's ring, which is empty by then; one that is cut at its
+  // start has shared memory of its own where that fits, else it goes through the workspace.
+  static constexpr bool HEAD_SMEM = RING + DEC_WARPS * HEAD + PARTS * (NH * 8 + 16) + 128 <= LIMIT;
+  static constexpr int HEADS = HEAD_SMEM ? DEC_WARPS * HEAD : 0;
+  static constexpr int SMEM = RING + HEADS + PARTS * (NH * 8 + 16) + 128;
+  static_assert(HEAD <= STAGES * STAGE, "a part fits the ring of a warp");
 };
 
 __device__ __forceinline__ void dec_cp16(uint32_t dst, const void* src, bool there) {
@@ -118,8 +124,8 @@ __device__ __forceinline__ uint32_t dec_pack_out(const DecodeParams& p, float x,
 
 // A stretch that a part in shared memory belongs to.
 struct DecPart {
-  long long s;  // where the stretch begins on the line; -1: no part
-  int b, hg, nt, pad;
+  int s;  // where the stretch begins on the line; -1: no part
+  int b, hg, nt;
 };
 
 template <int D, int KIND, int NT>
@@ -129,69 +135,58 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
   constexpr int KT = C::KS / 16, KSTEPS = D / 16, STAGES = C::STAGES, NH = C::NH, RPI = 32 / C::CH;
   constexpr bool BF = KIND == DEC_BF16;
   extern __shared__ __align__(128) uint8_t smem[];
-  float2* part_ml = reinterpret_cast<float2*>(smem + C::RING);                             // [part][head]
-  DecPart* parts = reinterpret_cast<DecPart*>(smem + C::RING + C::PARTS * NH * 8);          // [part]
-  // the head of the kernel borrows the ring
-  long long* sh_sum = reinterpret_cast<long long*>(smem);     // [warp]
-  long long* sh_rem = sh_sum + DEC_WARPS;                     // [warp]
-  int* sh_b = reinterpret_cast<int*>(sh_rem + DEC_WARPS);     // [warp]
+  float2* part_ml = reinterpret_cast<float2*>(smem + C::RING + C::HEADS);                  // [part][head]
+  DecPart* parts = reinterpret_cast<DecPart*>(smem + C::RING + C::HEADS + C::PARTS * NH * 8);  // [part]
+  int* sh_sum = reinterpret_cast<int*>(parts + C::PARTS);                                  // [warp]
+  int4* sh_at = reinterpret_cast<int4*>(sh_sum + 2 * DEC_WARPS);  // [warp] where its piece begins: sequence, length, head group, tile
   const tb200_attention_decode_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int batch = (int)a.batch;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what ran before: it may still be ending while this starts
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // ---- this warp's piece of the line
+  // ---- this warp's piece of the line (its length fits 32 bits: the host has seen to it)
   const int chunk = (batch + DEC_WARPS * 32 - 1) / (DEC_WARPS * 32);
   const int b_lo = min((int)threadIdx.x * chunk, batch), b_hi = min(b_lo + chunk, batch);
-  long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += (long long)((dec_len(p, b) + C::KS - 1) / C::KS) * p.hgs;
-  long long upto = mine;
+  auto tiles_of = [](int len) { return (len + C::KS - 1) / C::KS; };
+  int mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += tiles_of(dec_len(p, b)) * p.hgs;
+  int upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+    const int o = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += o;
   }
   if (lane == 31) sh_sum[warp] = upto;
   __syncthreads();
-  long long total = 0;
+  int total = 0;
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) {
     if (w < warp) upto += sh_sum[w];
     total += sh_sum[w];
   }
-  const long long per = max((total + gridDim.x * DEC_WARPS - 1) / (gridDim.x * DEC_WARPS), 1ll);  // tiles of a warp
-  const long long cta_first = per * DEC_WARPS * blockIdx.x, cta_last = min(cta_first + per * DEC_WARPS, total);
-#pragma unroll
+  const uint32_t n_warps = gridDim.x * DEC_WARPS;
+  const int per = (int)max(((uint32_t)total + n_warps - 1) / n_warps, 1u);  // tiles of a warp
+  const int cta_first = (int)min((long long)per * DEC_WARPS * blockIdx.x, (long long)total);
+  const int cta_last = min(cta_first + per * DEC_WARPS, total);
   for (int w = 0; w < DEC_WARPS; ++w) {
-    const long long target = cta_first + per * w;
+    const int target = cta_first + per * w;
     if (target < upto && upto - mine <= target) {
-      long long at = upto - mine;
+      int at = upto - mine;
       for (int b = b_lo; b < b_hi; ++b) {
-        const long long n = (long long)((dec_len(p, b) + C::KS - 1) / C::KS) * p.hgs;
-        if (target < at + n) {
-          sh_b[w] = b;
-          sh_rem[w] = target - at;
+        const int len = dec_len(p, b), nt = tiles_of(len), rem = target - at;
+        if (rem < nt * p.hgs) {
+          const int hg = rem / nt;
+          sh_at[w] = make_int4(b, len, hg, rem - hg * nt);
           break;
         }
-        at += n;
+        at += nt * p.hgs;
       }
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.per = per * DEC_WARPS;
-  // sequences without a key
-  for (int b = blockIdx.x; b < batch; b += gridDim.x) {
-    if (dec_len(p, b) > 0) continue;
-    for (int i = threadIdx.x; i < (int)a.heads * (D / 2); i += blockDim.x)
-      reinterpret_cast<uint32_t*>(dec_out(p, b, i / (D / 2)))[i % (D / 2)] = 0u;
-    if (a.lse)
-      for (int h = threadIdx.x; h < (int)a.heads; h += blockDim.x) a.lse[(long long)b * a.heads + h] = -INFINITY;
-  }
-  if (cta_first >= cta_last) {
-    if (threadIdx.x == 0) p.meta[blockIdx.x].b = -1;
-    return;
-  }
-  const long long first = cta_first + per * warp, last = min(first + per, cta_last);
+  const int first = cta_first + per * warp, last = min(first + per, cta_last);
+  const bool works = first < last;
 
   // ---- positions on the line: one runs ahead for the loads, one for the products
   struct At {
@@ -201,7 +196,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
   auto enter = [&](At& x, int b, int len) {
     x.b = b;
     x.len = len;
-    x.nt = (len + C::KS - 1) / C::KS;
+    x.nt = tiles_of(len);
     x.next = b + 1 < batch ? dec_len(p, b + 1) : 0;
   };
   auto next_stretch = [&](At& x) {
@@ -213,22 +208,29 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     if (b < batch) enter(x, b, len);
   };
   At ld = {};
-  const bool works = first < last;
   if (works) {
-    const long long rem = sh_rem[warp];
-    enter(ld, sh_b[warp], dec_len(p, sh_b[warp]));
-    ld.hg = (int)(rem / ld.nt);
-    ld.t = (int)(rem - (long long)ld.hg * ld.nt);
+    const int4 x = sh_at[warp];
+    enter(ld, x.x, x.y);
+    ld.hg = x.z;
+    ld.t = x.w;
   }
   At cur = ld;
-  if (threadIdx.x == 0) p.meta[blockIdx.x] = DecMeta{cur.b, cur.hg, first - cur.t, first - cur.t + cur.nt};
-  __syncthreads();  // the ring is free from here on
   if (lane < 2) parts[2 * warp + lane].s = -1;
+  auto part_o = [&](int part) {
+    if (part & 1) return reinterpret_cast<float*>(smem + (part >> 1) * STAGES * C::STAGE);
+    if (C::HEAD_SMEM) return reinterpret_cast<float*>(smem + C::RING + (part >> 1) * C::HEAD);
+    return p.warp_o + ((long long)blockIdx.x * DEC_WARPS + (part >> 1)) * NH * D;
+  };
 
   const uint32_t ring = smem_u32(smem) + warp * STAGES * C::STAGE;
   const bool page_steps = a.page_size % C::KS == 0;  // then a step's keys lie in one page
   const int row0 = lane / C::CH, col0 = lane % C::CH * 16;
-  // Places of a step's rows: lane r looks up row r (page_steps: all lanes the step's first row), a step ahead of its copies.
+  // Places of a step's rows: lane r looks up row r (page_steps: all lanes the step's first row). The page table passes
+  // through a window of 64 entries in two registers, so a step finds its pages there without waiting for memory.
+  int win_b = -1, win0 = 0, win_lo = -1, win_hi = -1;
+  auto page_entry = [&](int slot) {
+    return slot < (int)a.max_pages && (long long)slot * a.page_size < ld.len ? a.page_table[ld.b * a.table_stride + slot] : -1;
+  };
   const uint8_t *k_at = nullptr, *v_at = nullptr;
   long long k_kvh = 0, v_kvh = 0;  // byte offsets of the kv head
   int rows = 0;                    // rows of the step that exist
@@ -242,11 +244,26 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     const int key0 = ld.t * C::KS;
     rows = min(ld.len - key0, C::KS);
     there = false;
+    auto slot_of = [&](int key) { return (int)(__umulhi((uint32_t)key * 2u, p.page_mul) >> p.page_shift); };
+    const int first_slot = slot_of(key0);
+    if (ld.b != win_b || first_slot < win0) {
+      win_b = ld.b;
+      win0 = first_slot;
+      win_lo = page_entry(win0 + lane);
+      win_hi = page_entry(win0 + 32 + lane);
+    } else if (first_slot >= win0 + 32) {  // a step never moves on by more than 32 pages
+      win0 += 32;
+      win_lo = win_hi;
+      win_hi = page_entry(win0 + 32 + lane);
+    }
     const int r = page_steps ? 0 : lane % C::KS;
+    const int key = key0 + r, slot = slot_of(key), in_page = key - slot * a.page_size;
+    int page = __shfl_sync(0xffffffffu, win_lo, (slot - win0) & 31);
+    if (!page_steps) {
+      const int high = __shfl_sync(0xffffffffu, win_hi, (slot - win0) & 31);
+      if (slot - win0 >= 32) page = high;
+    }
     if (r < rows) {
-      const int key = key0 + r, slot = (int)(__umulhi((uint32_t)key * 2u, p.page_mul) >> p.page_shift);
-      const int in_page = key - slot * a.page_size;
-      const int page = a.page_table[ld.b * a.table_stride + slot];
       there = page >= 0 && page < (int)a.n_pages;
       k_at = (const uint8_t*)a.k_cache + page * p.k_page + in_page * p.k_tok + k_kvh;
       v_at = (const uint8_t*)a.v_cache + page * p.v_page + in_page * p.v_tok + v_kvh;
@@ -290,7 +307,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
       dec_cp16(to + C::KS * C::ROW, ok ? vp + col0 : (const uint8_t*)a.v_cache, ok);
     }
   };
-  long long to_load = last - first;
+  int to_load = last - first;
   auto load_next = [&](int stage) {
     if (to_load > 0) {
       issue(stage);
@@ -373,17 +390,30 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     }
   };
   if (works) {
-    load_q(cur);
     enter_head();
     look_up();
+    load_q(cur);
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) load_next(s);
+  }
+
+  // ---- what nothing waits for: the join's view of this CTA, sequences without a key
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) *p.per = per * DEC_WARPS;
+    p.meta[blockIdx.x] = DecMeta{works ? cur.b : -1, cur.hg, first - cur.t, first - cur.t + cur.nt};
+  }
+  for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+    if (dec_len(p, b) > 0) continue;
+    for (int i = threadIdx.x; i < (int)a.heads * (D / 2); i += blockDim.x)
+      reinterpret_cast<uint32_t*>(dec_out(p, b, i / (D / 2)))[i % (D / 2)] = 0u;
+    if (a.lse)
+      for (int h = threadIdx.x; h < (int)a.heads; h += blockDim.x) a.lse[(long long)b * a.heads + h] = -INFINITY;
   }
 
   // ---- the loop
   bool fresh = true;
   int stage = 0;
-  for (long long at = first; at < last; ++at) {
+  for (int at = first; at < last; ++at) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();
     load_next(stage == 0 ? STAGES - 1 : stage - 1);
@@ -502,7 +532,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     if (++cur.t < cur.nt && at + 1 < last) continue;
 
     // ---- end of a stretch or of the piece
-    const long long s0 = at + 1 - cur.t;  // where the stretch begins on the line
+    const int s0 = at + 1 - cur.t;  // where the stretch begins on the line
     const int b = cur.b, out_head = head0, out_heads = heads, out_kvh = kvh;
     const bool whole = cur.t == cur.nt && s0 >= first;
     const int done_hg = cur.hg, done_nt = cur.nt;
@@ -547,10 +577,14 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
         }
       }
     } else {
-      // cut at the piece's start (part 2 w) or, begun here, at its end (part 2 w + 1)
-      const int part = 2 * warp + (s0 >= first ? 1 : 0);
-      if (lane == 0) parts[part] = DecPart{s0, b, done_hg, done_nt, 0};
-      float* dst = p.warp_o + ((long long)blockIdx.x * C::PARTS + part) * NH * D;
+      // part 2 w ends in this piece, part 2 w + 1 reaches its end
+      const int part = 2 * warp + (at + 1 < last ? 0 : 1);
+      if (lane == 0) parts[part] = DecPart{s0, b, done_hg, done_nt};
+      float* dst = part_o(part);
+      if (part & 1) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -570,22 +604,18 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
     }
   }
 
-  // ---- merge the parts of this CTA, stretch by stretch (they lie in the order of the line)
+  // ---- merge the parts of this CTA, stretch by stretch (they lie in the order of the line), a warp per head
   __syncthreads();
-  for (int i = 0; i < C::PARTS;) {
-    const DecPart me = parts[i];
-    if (me.s < 0) {
-      ++i;
-      continue;
-    }
-    int n = 1;  // parts i .. i + n - 1, without the empty ones, belong to this stretch
-    while (i + n < C::PARTS && (parts[i + n].s < 0 || parts[i + n].s == me.s)) ++n;
+  auto merge = [&](int i, int n, const DecPart& me, int turn) {  // parts i .. i + n - 1, without the empty ones
     const bool whole = me.s >= cta_first && me.s + me.nt <= cta_last;
-    const int slot = me.s >= cta_first ? 1 : 0;
     const int of_kv = me.hg / p.groups_per_kv, from = of_kv * p.group + (me.hg - of_kv * p.groups_per_kv) * NH;
     const int n_heads = min(NH, (of_kv + 1) * p.group - from);
-    for (int e = threadIdx.x; e < n_heads * (D / 4); e += DEC_WARPS * 32) {
-      const int h = e / (D / 4), col = e % (D / 4) * 4;
+    const long long row = ((long long)blockIdx.x * 2 + (me.s >= cta_first ? 1 : 0)) * NH;
+    const float v_scale = KIND == DEC_E4M3 && whole ? a.v_scale[a.v_scale_n > 1 ? of_kv : 0] : 1.f;
+    constexpr int HPW = D == 64 ? 2 : 1;  // heads at a time
+    for (int h = (warp + turn) % DEC_WARPS * HPW + lane / (32 / HPW); h < n_heads; h += DEC_WARPS * HPW)
+#pragma unroll
+    for (int col = lane % (D / 4) * 4; col < D; col += 128) {
       float top = -INFINITY, sum = 0.f;
       for (int q = i; q < i + n; ++q)
         if (parts[q].s >= 0) top = fmaxf(top, part_ml[q * NH + h].x);
@@ -593,9 +623,8 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
       for (int q = i; q < i + n; ++q) {
         if (parts[q].s < 0) continue;
         const float2 ml = part_ml[q * NH + h];
+        const float4 v = *reinterpret_cast<const float4*>(part_o(q) + h * D + col);
         const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-        const float4 v =
-            *reinterpret_cast<const float4*>(p.warp_o + (((long long)blockIdx.x * C::PARTS + q) * NH + h) * D + col);
         sum += f * ml.y;
         x.x += f * v.x;
         x.y += f * v.y;
@@ -603,48 +632,65 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
         x.w += f * v.w;
       }
       if (whole) {
-        float inv = sum == 0.f ? 0.f : 1.f / sum;
-        if (KIND == DEC_E4M3) inv *= a.v_scale[a.v_scale_n > 1 ? of_kv : 0];
+        const float inv = sum == 0.f ? 0.f : v_scale / sum;
         *reinterpret_cast<uint2*>(dec_out(p, me.b, from + h) + col) =
             make_uint2(dec_pack_out(p, x.x * inv, x.y * inv), dec_pack_out(p, x.z * inv, x.w * inv));
         if (a.lse && col == 0) a.lse[(long long)me.b * a.heads + from + h] = top + log2f(sum);
       } else {
-        const long long part = ((long long)blockIdx.x * 2 + slot) * NH + h;
-        *reinterpret_cast<float4*>(p.part_o + part * D + col) = x;
-        if (col == 0) p.part_ml[part] = make_float2(top, sum);
+        *reinterpret_cast<float4*>(p.part_o + (row + h) * D + col) = x;
+        if (col == 0) p.part_ml[row + h] = make_float2(top, sum);
       }
+    }
+  };
+  for (int i = 0, turn = 0; i < C::PARTS;) {
+    const DecPart me = parts[i];
+    int n = 1;
+    if (me.s >= 0) {
+      while (i + n < C::PARTS && (parts[i + n].s < 0 || parts[i + n].s == me.s)) ++n;
+      merge(i, n, me, turn++);
     }
     i += n;
   }
 }
 
 // Joins the parts of the stretch that is cut at the start of CTA blockIdx.x's piece for the first time: the end of the
-// CTA before, then the beginning of every CTA that it reaches into. One block per query head of the group.
+// CTA before, then the beginning of every CTA that it reaches into. One block per query head of the group; the first
+// parts are loaded before their weights are known, for the kernel is a chain of loads and little else.
+static constexpr int JOIN_THREADS = 128;
 template <int D, int NH>
-__global__ void __launch_bounds__(128) attention_decode_join_kernel(const __grid_constant__ DecodeParams p, int ctas, int e4m3) {
-  constexpr int COLS = D / 4, LANES = 128 / COLS;  // threads along a row, rows at a time
+__global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const __grid_constant__ DecodeParams p, int e4m3) {
+  constexpr int COLS = D / 4, LANES = JOIN_THREADS / COLS;  // threads along a row, rows at a time
+  constexpr int EARLY = 4, WARPS = JOIN_THREADS / 32;
   __shared__ float weight[1024];
-  __shared__ float red[4], red2[4];
-  __shared__ float4 acc[128];
+  __shared__ float red[2][WARPS];
+  __shared__ float4 acc[JOIN_THREADS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x, h = blockIdx.y;
   const DecMeta me = p.meta[c];
-  const long long per = *p.per;
+  const int per = *p.per;
   if (me.b < 0 || me.s >= per * c || me.s < per * (c - 1)) return;
   const int kvh = me.hg / p.groups_per_kv, head = kvh * p.group + me.hg % p.groups_per_kv * NH + h;
   if (head >= (kvh + 1) * p.group) return;
-  const int parts = 1 + (int)((me.e + per - 1) / per) - c;  // at most ctas, which is at most 1024
+  const int parts = 1 + (me.e - 1) / per + 1 - c;  // at most the CTAs, which are at most 1024
   auto part_of = [&](int i) { return i == 0 ? ((long long)(c - 1) * 2 + 1) * NH + h : (long long)(c + i - 1) * 2 * NH + h; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = threadIdx.x % COLS, from = threadIdx.x / COLS;
+  auto load = [&](int i) {
+    return i < parts ? reinterpret_cast<const float4*>(p.part_o + part_of(i) * D)[col] : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float4 early[EARLY];
+#pragma unroll
+  for (int u = 0; u < EARLY; ++u) early[u] = load(from + u * LANES);
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += 128) top = fmaxf(top, p.part_ml[part_of(i)].x);
+  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) top = fmaxf(top, p.part_ml[part_of(i)].x);
 #pragma unroll
   for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-  if (lane == 0) red[warp] = top;
+  if (lane == 0) red[0][warp] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[0][w]);
   float sum = 0.f;
-  for (int i = threadIdx.x; i < parts; i += 128) {
+  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
     const float2 ml = p.part_ml[part_of(i)];
     const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
     weight[i] = f;
@@ -652,30 +698,27 @@ __global__ void __launch_bounds__(128) attention_decode_join_kernel(const __grid
   }
 #pragma unroll
   for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-  if (lane == 0) red2[warp] = sum;
+  if (lane == 0) red[1][warp] = sum;
   __syncthreads();
-  sum = (red2[0] + red2[1]) + (red2[2] + red2[3]);
-  const int col = threadIdx.x % COLS, from = threadIdx.x / COLS;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) sum += red[1][w];
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = from; i < parts; i += LANES) {
-    const float f = weight[i];
-    const float4 v = reinterpret_cast<const float4*>(p.part_o + part_of(i) * D)[col];
+  auto add = [&](float f, const float4& v) {
     x.x += f * v.x;
     x.y += f * v.y;
     x.z += f * v.z;
     x.w += f * v.w;
-  }
+  };
+#pragma unroll
+  for (int u = 0; u < EARLY; ++u)
+    if (from + u * LANES < parts) add(weight[from + u * LANES], early[u]);
+#pragma unroll 8
+  for (int i = from + EARLY * LANES; i < parts; i += LANES) add(weight[i], load(i));
   acc[threadIdx.x] = x;
   __syncthreads();
   if (from == 0) {
-    for (int i = 1; i < LANES; ++i) {
-      const float4 v = acc[i * COLS + col];
-      x.x += v.x;
-      x.y += v.y;
-      x.z += v.z;
-      x.w += v.w;
-    }
+    for (int i = 1; i < LANES; ++i) add(1.f, acc[i * COLS + col]);
     float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (e4m3) inv *= p.a.v_scale[p.a.v_scale_n > 1 ? kvh : 0];
     *reinterpret_cast<uint2*>(dec_out(p, me.b, head) + col * 4) =
@@ -697,7 +740,7 @@ static DecPlan dec_plan(const tb200_attention_decode_args* a, int sms) {
   d.ctas = sms * (a->head_dim == 256 ? 1 : 2);
   const size_t parts = (size_t)d.ctas * 2 * d.nh;
   d.off_warp = parts * a->head_dim * sizeof(float);
-  d.off_ml = d.off_warp + parts * DEC_WARPS * a->head_dim * sizeof(float);
+  d.off_ml = d.off_warp + parts / 2 * DEC_WARPS * a->head_dim * sizeof(float);
   d.off_meta = d.off_ml + parts * sizeof(float2);
   d.off_per = d.off_meta + (size_t)d.ctas * sizeof(DecMeta);
   d.bytes = d.off_per + 16;
@@ -707,21 +750,25 @@ static DecPlan dec_plan(const tb200_attention_decode_args* a, int sms) {
 template <int D, int KIND, int NT>
 static int launch_decode(const DecodeParams& p, int ctas, cudaStream_t stream) {
   using C = DecCfg<D, KIND, NT>;
-  static_assert(C::STAGES >= 3 && C::CTAS * (C::SMEM + 1024) <= 233472, "shared memory budget");
+  static_assert(C::STAGES >= 3 && C::SMEM <= C::LIMIT, "shared memory budget");
   auto kfn = attention_decode_kernel<D, KIND, NT>;
   if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TB200_ERR_CUDA;
-  kfn<<<ctas, DEC_WARPS * 32, C::SMEM, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
+  // Both start while the kernel before them ends, and wait for it before they read anything.
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, C::NH);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(DEC_WARPS * 32);
+  cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_err(cudaLaunchKernelEx(&cfg, attention_decode_join_kernel<D, C::NH>, p, ctas, (int)(KIND == DEC_E4M3)));
+  if (cudaLaunchKernelEx(&cfg, kfn, p) != cudaSuccess) return TB200_ERR_CUDA;
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)(p.group < C::NH ? p.group : C::NH));
+  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.dynamicSmemBytes = 0;
+  return cuda_err(cudaLaunchKernelEx(&cfg, attention_decode_join_kernel<D, C::NH>, p, (int)(KIND == DEC_E4M3)));
 }
 
 template <int D, int KIND>
@@ -787,7 +834,9 @@ extern "C" int tb200_attention_decode(const tb200_attention_decode_args* a, void
   const int sms = sm_count();
   if (sms <= 0) return TB200_ERR_CUDA;
   const DecPlan plan = dec_plan(a, sms);
-  if (plan.ctas > 1024) return TB200_ERR_UNSUPPORTED;
+  const int64_t group = a->heads / a->kv_heads, hgs = (group + plan.nh - 1) / plan.nh * a->kv_heads;
+  const int64_t tiles = (a->max_pages * a->page_size + 15) / 16;  // of one sequence and head group, at most
+  if (plan.ctas > 1024 || hgs * tiles > INT32_MAX || a->batch * (hgs * tiles) > INT32_MAX - (1 << 20)) return TB200_ERR_UNSUPPORTED;
   if (!a->workspace || off16(a->workspace) || a->workspace_bytes < plan.bytes) return TB200_ERR_BAD_ARG;
   DecodeParams p;
   memset(&p, 0, sizeof(p));
@@ -811,7 +860,7 @@ extern "C" int tb200_attention_decode(const tb200_attention_decode_args* a, void
   p.warp_o = reinterpret_cast<float*>(ws + plan.off_warp);
   p.part_ml = reinterpret_cast<float2*>(ws + plan.off_ml);
   p.meta = reinterpret_cast<DecMeta*>(ws + plan.off_meta);
-  p.per = reinterpret_cast<long long*>(ws + plan.off_per);
+  p.per = reinterpret_cast<int*>(ws + plan.off_per);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   return a->head_dim == 64 ? launch_decode_kind<64>(p, plan, stream)
          : a->head_dim == 128 ? launch_decode_kind<128>(p, plan, stream) : launch_decode_kind<256>(p, plan, stream);
