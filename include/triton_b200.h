@@ -294,7 +294,7 @@ int tb200_attention_bwd(const tb200_attention_bwd_args* args, void* stream);
  * Tokens at or past cu_seqlens[batch]: nothing is written. A position below 0, at or past n_positions, or past the page
  * table: the rows of q_out and k_out are zeros, the cache is left alone.
  * head_dim 64, 128 or 256; rotary_dim a multiple of 16, at most head_dim; dtype TB200_BF16 or TB200_F16. All bases 16-byte
- * aligned, all strides multiples of 8 elements (an e4m3 cache: 8-byte aligned, multiples of 8).
+ * aligned, rot_stride a multiple of 4, all other strides multiples of 8 elements (an e4m3 cache: 8-byte aligned, multiples of 8).
  */
 typedef struct {
   const void* q;

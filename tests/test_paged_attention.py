@@ -191,7 +191,9 @@ def test_append_strided_in_place_and_without_queries(cuda):
     odd = torch.empty(12 * 2 * 64 + 1, dtype=BF16, device=cuda)[1:].view(12, 2, 64)  # rows off the 16-byte grid are copied
     odd.copy_(k0)
     cache.k.copy_(before[0]), cache.v.copy_(before[1])
-    assert fa().append_paged_kv(None, odd, v0, cache.k, cache.v, cache.table, cache.seq_lens, cu, cos=cos, sin=sin) is None
+    off = torch.empty(40 * 32 + 1, device=cuda)[1:].view(40, 32)
+    off.copy_(cos)  # a table off the grid too
+    assert fa().append_paged_kv(None, odd, v0, cache.k, cache.v, cache.table, cache.seq_lens, cu, cos=off, sin=sin) is None
     assert torch.equal(cache.k.view(torch.int16), first[0].view(torch.int16))
     assert torch.equal(cache.v.view(torch.int16), first[1].view(torch.int16))
 
@@ -685,7 +687,7 @@ def filled(cls, **kw):
     (dict(page_size=0), -1), (dict(cu_seqlens=None, tokens=3), -1), (dict(head_dim=96), -2), (dict(dtype=2), -2),
     (dict(cache_dtype=1), -2), (dict(cache_dtype=4), -2), (dict(cache_dtype=3, k_scale=None), -1), (dict(cache_dtype=3, k_scale_n=3), -1),
     (dict(rotary_dim=24), -1), (dict(rotary_dim=144), -1), (dict(q=4104), -1), (dict(k_cache=4100), -1), (dict(kc_stride_tok=100), -1),
-    (dict(tokens=1 << 32), -2), (dict(tokens=0), 0)])
+    (dict(cos=4100), -1), (dict(rot_stride=6), -1), (dict(tokens=1 << 32), -2), (dict(tokens=0), 0)])
 def test_append_refusals(lib, change, code):
     from triton_b200 import _lib
     assert lib.tb200_kv_append(ctypes.byref(filled(_lib.KvAppendArgs, **change)), None) == code

@@ -753,22 +753,10 @@ static int launch_decode(const DecodeParams& p, int ctas, cudaStream_t stream) {
   static_assert(C::STAGES >= 3 && C::SMEM <= C::LIMIT, "shared memory budget");
   auto kfn = attention_decode_kernel<D, KIND, NT>;
   if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TB200_ERR_CUDA;
-  // Both start while the kernel before them ends, and wait for it before they read anything.
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(DEC_WARPS * 32);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kfn, p) != cudaSuccess) return TB200_ERR_CUDA;
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)(p.group < C::NH ? p.group : C::NH));
-  cfg.blockDim = dim3(JOIN_THREADS);
-  cfg.dynamicSmemBytes = 0;
-  return cuda_err(cudaLaunchKernelEx(&cfg, attention_decode_join_kernel<D, C::NH>, p, (int)(KIND == DEC_E4M3)));
+  if (launch_overlapped(kfn, dim3((unsigned)ctas), DEC_WARPS * 32, C::SMEM, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  const dim3 join((unsigned)ctas, (unsigned)(p.group < C::NH ? p.group : C::NH));
+  return cuda_err(
+      launch_overlapped(attention_decode_join_kernel<D, C::NH>, join, JOIN_THREADS, 0, stream, p, (int)(KIND == DEC_E4M3)));
 }
 
 template <int D, int KIND>

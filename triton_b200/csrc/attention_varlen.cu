@@ -659,17 +659,7 @@ static int launch_varlen(const VarlenParams& p, bool f16, int grid, cudaStream_t
   if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
     return TB200_ERR_CUDA;
   // starts while the schedule is being made: barriers and tensor memory are set up by the time it is there
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(VAR_THREADS);
-  cfg.dynamicSmemBytes = L::TOTAL;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cuda_err(cudaLaunchKernelEx(&cfg, kfn, p));
+  return cuda_err(launch_overlapped(kfn, dim3((unsigned)grid), VAR_THREADS, L::TOTAL, stream, p));
 }
 
 struct VarPlan {

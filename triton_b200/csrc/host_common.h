@@ -21,6 +21,24 @@ int encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int rank, const voi
                 const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle,
                 CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
+// Launches a kernel that may start while the one before it in the stream ends. The kernel executes griddepcontrol.wait
+// in every block before it reads or writes global memory: until then nothing of the work before it is complete.
+template <typename Kernel, typename... Args>
+inline cudaError_t launch_overlapped(Kernel kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                                     const Args&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 inline int cuda_err(cudaError_t e) { return e == cudaSuccess ? TB200_OK : TB200_ERR_CUDA; }
 
 }  // namespace tb200

@@ -78,11 +78,35 @@ template <int D, bool F16, bool C8, int U>
 __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int LPR = D / 16, RPW = 32 / LPR;
   const tb200_kv_append_args& a = p.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int64_t gw = (int64_t)blockIdx.x * APP_WARPS + (threadIdx.x >> 5);
-  const int64_t t = gw / p.tasks_per_token;
-  if (t >= a.tokens) return;
+  const uint32_t gw = blockIdx.x * APP_WARPS + (threadIdx.x >> 5);
+  const uint32_t t = gw / (uint32_t)p.tasks_per_token;
+  if (t >= (uint32_t)a.tokens) return;
   const int row0 = (int)(gw - t * p.tasks_per_token) * (RPW * U) + lane / LPR;
+  const int n_q = a.q ? (int)a.heads : 0, n_kv = (int)a.kv_heads;
+
+  // ---- this lane's two chunks of 8 columns
+  const int item = lane % LPR, rot = a.cos ? a.rotary_dim : 0;
+  const bool turns = item * 16 < rot;
+  const bool halves = turns && !a.interleaved;
+  const int c0 = halves ? item * 8 : item * 16;
+  const int c1 = halves ? c0 + rot / 2 : c0 + 8;
+
+  // ---- all rows first: where they go takes a chain of look-ups
+  uint4 w0[U], w1[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int row = row0 + u * RPW;
+    w0[u] = w1[u] = make_uint4(0, 0, 0, 0);
+    if (row < p.rows) {
+      const uint16_t* src = row < n_q ? (const uint16_t*)a.q + t * a.q_stride_tok + row * a.q_stride_head
+                            : row < n_q + n_kv ? (const uint16_t*)a.k + t * a.k_stride_tok + (row - n_q) * a.k_stride_head
+                                               : (const uint16_t*)a.v + t * a.v_stride_tok + (row - n_q - n_kv) * a.v_stride_head;
+      w0[u] = *reinterpret_cast<const uint4*>(src + c0);
+      w1[u] = *reinterpret_cast<const uint4*>(src + c1);
+    }
+  }
 
   // ---- the token's sequence, position, table row and page
   int b = (int)t, pos;
@@ -90,7 +114,7 @@ __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_
     b = find_sequence(a.cu_seqlens, (int)a.batch, (int)t, lane);
     if (b < 0) return;
     const int end = a.cu_seqlens[b + 1];
-    if (t >= end) return;  // behind the last sequence
+    if ((int)t >= end) return;  // behind the last sequence
     pos = a.seq_lens[b] - (end - (int)t);
   } else {
     pos = a.seq_lens[b] - 1;
@@ -101,24 +125,17 @@ __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_
   if (valid) page = a.page_table[b * a.table_stride + slot];
   const bool cached = page >= 0 && page < a.n_pages;
   const int in_page = valid ? pos - slot * a.page_size : 0;
-
-  // ---- this lane's two chunks of 8 columns, and the angles of its 8 pairs
-  const int item = lane % LPR, rot = a.cos ? a.rotary_dim : 0;
-  const bool turns = item * 16 < rot;
-  const bool halves = turns && !a.interleaved;
-  const int c0 = halves ? item * 8 : item * 16;
-  const int c1 = halves ? c0 + rot / 2 : c0 + 8;
-  float cs[8], sn[8];
+  float cs[8], sn[8];  // the angles of this lane's 8 pairs
   if (turns && valid) {
-    const float* cr = a.cos + pos * a.rot_stride + item * 8;
-    const float* sr = a.sin + pos * a.rot_stride + item * 8;
+    const float4* cr = reinterpret_cast<const float4*>(a.cos + pos * a.rot_stride + item * 8);
+    const float4* sr = reinterpret_cast<const float4*>(a.sin + pos * a.rot_stride + item * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      cs[i] = cr[i];
-      sn[i] = sr[i];
+    for (int i = 0; i < 2; ++i) {
+      const float4 c = cr[i], s = sr[i];
+      cs[4 * i] = c.x, cs[4 * i + 1] = c.y, cs[4 * i + 2] = c.z, cs[4 * i + 3] = c.w;
+      sn[4 * i] = s.x, sn[4 * i + 1] = s.y, sn[4 * i + 2] = s.z, sn[4 * i + 3] = s.w;
     }
   }
-  const int n_q = a.q ? (int)a.heads : 0, n_kv = (int)a.kv_heads;
 
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -126,17 +143,10 @@ __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_
     if (row >= p.rows) break;
     const int which = row < n_q ? 0 : row < n_q + n_kv ? 1 : 2;
     const int h = which == 0 ? row : which == 1 ? row - n_q : row - n_q - n_kv;
-    const uint16_t* src = which == 0   ? (const uint16_t*)a.q + t * a.q_stride_tok + h * a.q_stride_head
-                          : which == 1 ? (const uint16_t*)a.k + t * a.k_stride_tok + h * a.k_stride_head
-                                       : (const uint16_t*)a.v + t * a.v_stride_tok + h * a.v_stride_head;
-    uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+    if (!valid) w0[u] = w1[u] = make_uint4(0, 0, 0, 0);
     float x[8], y[8];
-    if (valid) {
-      w0 = *reinterpret_cast<const uint4*>(src + c0);
-      w1 = *reinterpret_cast<const uint4*>(src + c1);
-    }
-    widen8<F16>(w0, x);
-    widen8<F16>(w1, y);
+    widen8<F16>(w0[u], x);
+    widen8<F16>(w1[u], y);
     if (which < 2 && turns && valid) {
       if (halves) {
 #pragma unroll
@@ -156,15 +166,15 @@ __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_
           y[2 * i] = r;
         }
       }
-      w0 = narrow8<F16>(x);
-      w1 = narrow8<F16>(y);
+      w0[u] = narrow8<F16>(x);
+      w1[u] = narrow8<F16>(y);
     }
     uint16_t* packed = which == 0                ? (uint16_t*)a.q_out + t * a.qo_stride_tok + h * a.qo_stride_head
                        : which == 1 && a.k_out ? (uint16_t*)a.k_out + t * a.ko_stride_tok + h * a.ko_stride_head
                                                  : nullptr;
     if (packed) {
-      *reinterpret_cast<uint4*>(packed + c0) = w0;
-      *reinterpret_cast<uint4*>(packed + c1) = w1;
+      *reinterpret_cast<uint4*>(packed + c0) = w0[u];
+      *reinterpret_cast<uint4*>(packed + c1) = w1[u];
     }
     if (which > 0 && cached) {
       const int64_t at = which == 1
@@ -179,8 +189,8 @@ __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_
         *reinterpret_cast<uint2*>(dst + c1) = narrow8_e4m3(y, scale);
       } else {
         uint16_t* dst = (uint16_t*)pool + at;
-        *reinterpret_cast<uint4*>(dst + c0) = w0;
-        *reinterpret_cast<uint4*>(dst + c1) = w1;
+        *reinterpret_cast<uint4*>(dst + c0) = w0[u];
+        *reinterpret_cast<uint4*>(dst + c1) = w1[u];
       }
     }
   }
@@ -192,9 +202,8 @@ static int launch_append(const AppendParams& p, cudaStream_t stream) {
   auto kfn = f16 ? (c8 ? kv_append_kernel<D, true, true, U> : kv_append_kernel<D, true, false, U>)
                  : (c8 ? kv_append_kernel<D, false, true, U> : kv_append_kernel<D, false, false, U>);
   const int64_t blocks = (p.a.tokens * p.tasks_per_token + APP_WARPS - 1) / APP_WARPS;
-  if (blocks > INT32_MAX) return TB200_ERR_UNSUPPORTED;
-  kfn<<<(unsigned)blocks, APP_WARPS * 32, 0, stream>>>(p);
-  return cuda_err(cudaGetLastError());
+  if (blocks * APP_WARPS > INT32_MAX) return TB200_ERR_UNSUPPORTED;
+  return cuda_err(launch_overlapped(kfn, dim3((unsigned)blocks), APP_WARPS * 32, 0, stream, p));
 }
 
 }  // namespace tb200
@@ -221,7 +230,7 @@ extern "C" int tb200_kv_append(const tb200_kv_append_args* a, void* stream_) {
   if (a->tokens > INT32_MAX || a->batch > INT32_MAX - 1 || a->heads > (1 << 20) || a->kv_heads > (1 << 20))
     return TB200_ERR_UNSUPPORTED;
   if (misaligned(a->q, 16) || misaligned(a->k, 16) || misaligned(a->v, 16) || misaligned(a->q_out, 16) ||
-      misaligned(a->k_out, 16) || misaligned(a->k_cache, c8 ? 8 : 16) || misaligned(a->v_cache, c8 ? 8 : 16))
+      misaligned(a->k_out, 16) || misaligned(a->cos, 16) || misaligned(a->sin, 16) || a->rot_stride % 4 || misaligned(a->k_cache, c8 ? 8 : 16) || misaligned(a->v_cache, c8 ? 8 : 16))
     return TB200_ERR_BAD_ARG;
   const int64_t strides[] = {a->q_stride_tok,  a->q_stride_head,  a->k_stride_tok,  a->k_stride_head,
                              a->v_stride_tok,  a->v_stride_head,  a->qo_stride_tok, a->qo_stride_head,

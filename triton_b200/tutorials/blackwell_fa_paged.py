@@ -145,15 +145,27 @@ def _check_cache(k_cache, v_cache, page_table, seq_lens, k_scale, v_scale, idx, 
             _lib.E4M3 if fp8 else _DT[dtype])
 
 
+def _aligned(t):
+    """A table as the kernels read it, 16 bytes at a time."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(fn, args, idx, name):
+def _call(name, args, idx, rows=None):
+    """Launches on the current stream of the data's device; `rows`: any tensor there, to allocate the call's workspace from."""
+    lib, ref = _lib.lib(), ctypes.byref(args)
     with _lib.device_guard(idx):
-        rc = fn(ctypes.byref(args), _lib.current_stream_ptr(idx))
+        if rows is not None:
+            need = getattr(lib, name[0])(ref)
+            ws = rows.new_empty(need // 2 + 1)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        rc = getattr(lib, name[-1])(ref, _lib.current_stream_ptr(idx))
     if rc:
-        _lib.check(rc, name)
+        _lib.check(rc, name[-1])
 
 
 def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, *, cos=None, sin=None,
@@ -193,7 +205,7 @@ def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=
     if cos is not None:
         assert cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
         assert cos.get_device() == sin.get_device() == idx
-        cos, sin = cos.contiguous(), sin.contiguous()
+        cos, sin = _aligned(cos), _aligned(sin)
         positions, half = cos.shape
         assert 0 < 2 * half <= d and half % 8 == 0, "rotary_dim: a multiple of 16, at most head_dim"
     qo, qos, qoh = (None, 0, 0) if q is None else _out_rows(q_out, q, "q_out")
@@ -207,7 +219,7 @@ def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=
         tokens, batch, 0 if q is None else heads, kv_heads, qs, qh, ks, kh, vs, vh, qos, qoh, kos, koh, *kst, *vst,
         table_stride, half, n_pages, max_pages, positions, page_size, d, 2 * half, 1 if interleaved else 0, _DT[dtype], cache_dt,
         kn, vn)
-    _call(_lib.lib().tb200_kv_append, args, idx, "tb200_kv_append")
+    _call(("tb200_kv_append", ), args, idx)
     return qo
 
 
@@ -227,12 +239,7 @@ def _decode(q, k_cache, v_cache, page_table, seq_lens, sm_scale, k_scale, v_scal
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _ptr(lse), page_table.data_ptr(),
         seq_lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), None, 0, batch, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
         table_stride, n_pages, max_pages, page_size, d, _DT[dtype], cache_dt, kn, vn, float(sm_scale))
-    lib = _lib.lib()
-    with _lib.device_guard(idx):
-        need = lib.tb200_attention_decode_workspace_bytes(ctypes.byref(args))
-    ws = q.new_empty(need // 2 + 1)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _call(lib.tb200_attention_decode, args, idx, "tb200_attention_decode")
+    _call(("tb200_attention_decode_workspace_bytes", "tb200_attention_decode"), args, idx, q)
     return o, lse
 
 
@@ -257,12 +264,7 @@ def _varlen(what, q, k, v, kst, vst, cu_q, cu_k, page_table, seq_lens, tokens_k,
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), cu_q.data_ptr(), _ptr(cu_k), _ptr(page_table),
         _ptr(seq_lens), None, 0, tokens, tokens_k, cu_q.shape[0] - 1, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
         table_stride, n_pages, max_pages, page_size, d, _DT[q.dtype], 1 if causal else 0, float(sm_scale))
-    lib = _lib.lib()
-    with _lib.device_guard(idx):
-        need = lib.tb200_attention_varlen_workspace_bytes(ctypes.byref(args))
-    ws = q.new_empty(need // 2 + 1)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _call(lib.tb200_attention_varlen_fwd, args, idx, "tb200_attention_varlen_fwd")
+    _call(("tb200_attention_varlen_workspace_bytes", "tb200_attention_varlen_fwd"), args, idx, q)
     return o, lse
 
 
