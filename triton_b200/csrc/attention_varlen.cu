@@ -4,15 +4,18 @@
 // The pipeline is that of attention.cu (warp 0 TMA loads, warp 1 issues every tcgen05.mma, two softmax warpgroups of 128
 // query rows that alternate on the tensor pipe; S and P in tensor memory, O rescaled only when the running maximum grew
 // by more than 2^8). What differs:
-//   rows      A group's 128 rows are 128 / gp consecutive tokens x gp query heads of one kv head (gp = the largest power
-//             of two in heads / kv_heads): one box of a 4-D tensor map (column, head of the pack, token, pack). A tile so
-//             covers fewer tokens, which wastes less on short sequences and on the causal diagonal, and K / V are read
-//             once per pack instead of once per head.
-//   schedule  attention_varlen_schedule_kernel turns the sequence offsets into a list of tiles, the longest KV walks
-//             first; the lengths never pass through the host. CTAs take tiles from the list in rounds of alternating
-//             direction (the first round dealt from the long end, the second back, ...), which evens out their sums.
+//   rows      A group's 128 rows are 128 / gp consecutive tokens x gp query heads of one kv head, gp a divisor of
+//             heads / kv_heads: one box of a 4-D tensor map (column, head of the pack, token, pack). A tile so covers fewer
+//             tokens, which wastes less on short sequences and on the causal diagonal, and K / V are read once per pack
+//             instead of once per head.
+//   schedule  attention_varlen_schedule_kernel turns the sequence offsets into a list of pieces, the longest KV walks
+//             first; the lengths never pass through the host. The load warp of a CTA draws its next piece from a counter and
+//             hands it to the other roles through shared memory.
+//   split     A tile whose KV walk is longer than an even share of all work (few queries over a long cache, one sequence
+//             among short ones) becomes several pieces: each leaves its accumulator, maxima and sums in the workspace, and
+//             attention_varlen_join_kernel combines them in the order of the keys.
 //   tails     The last KV block of a sequence runs into the next sequence's rows (or into whatever a page holds). Scores
-//             there are replaced by -inf, so K's content is irrelevant; V's is not (0 * NaN), so warps 2 and 3 overwrite
+//             there are replaced by -inf, so K's content is irrelevant; V's is not (0 * NaN), so warp 2 overwrites
 //             those rows of the V tile with zeros in shared memory before the P V product may read it.
 //   half      A tile whose tokens fit the first group (short sequences, ends) leaves the second group out.
 //   pages     A KV block is 128 / r boxes of r = gcd(page size, 128) rows; the lanes of the load warp look up and issue one
@@ -30,12 +33,23 @@ static constexpr int VAR_BN = 128;      // kv rows per block
 static constexpr int VAR_MAX_STAGES = 4;
 static constexpr float VAR_RESCALE_THRESHOLD = 8.0f;
 
-// One tile of the schedule (32 bytes): n_tok tokens from packed row tok0 on; diag = the last key position that token 0
-// of the tile sees under a causal mask; n0 / n1 = KV blocks of the first / second group (n1 = 0: no tokens in it).
-struct VarTile {
-  int tok0, n_tok, kv_len, kv_first, diag, n0, n1, pad;
+// One piece of the schedule: n_tok tokens from packed row tok0 on over the KV blocks from j0 on; diag = the last key
+// position that token 0 of the tile sees under a causal mask; n0 / n1 = KV blocks of the first / second group (n1 = 0: no
+// tokens in it). part: this piece's slot in the workspace for the first pack, part_step slots further for each pack (part
+// < 0: the tile is in one piece). In shared memory `part` is that of the pack, and n0 = 0 ends the list.
+struct __align__(16) VarTile {
+  int tok0, n_tok, kv_len, kv_first;
+  int diag, n0, n1, j0;
+  int part, part_step, pack, pad;
 };
-static_assert(sizeof(VarTile) == 32, "two 16-byte loads");
+// A tile that was split: its parts lie at part + pack * n_parts + (0 .. n_parts - 1).
+struct __align__(16) VarSplit {
+  int tok0, n_tok, part, n_parts;
+};
+static constexpr int VAR_MIN_BLOCKS = 4;  // no piece is cut below this many KV blocks: starting one costs about two
+struct VarCounters {
+  int n_pieces, n_split, n_parts, next;
+};
 
 struct VarlenParams {
   CUtensorMap tmq;       // (D, gp, tokens, packs), box (64, gp, 128 / gp, 1), 128-byte swizzle
@@ -43,11 +57,14 @@ struct VarlenParams {
   void* o;
   float* lse;
   int* status;
-  const VarTile* tiles;
-  const int* n_tiles;
+  const VarTile* pieces;
+  const VarSplit* splits;
+  VarCounters* count;
+  float* part_o;    // [part][rows of a tile][D]
+  float2* part_ml;  // [part][rows of a tile]: maximum, sum
   const int32_t* page_table;
   long long table_stride, o_stride_tok, o_stride_head;
-  int heads, packs, lgp, packs_per_kv;
+  int heads, packs, gp, packs_per_kv;
   int page_size, box_rows, n_pages, max_pages;
   int no_page;  // first page coordinate behind the pool: reads as zeros
   int causal;
@@ -56,10 +73,12 @@ struct VarlenParams {
 
 struct ScheduleParams {
   const int32_t *cu_q, *cu_k, *seq_lens;
-  VarTile* tiles;
-  int* n_tiles;
-  int batch, tokens_q, tokens_k, cap, tile_tokens, group_tokens, causal, two_groups, paged;
+  VarTile* pieces;
+  VarSplit* splits;
+  VarCounters* count;
+  int batch, tokens_q, tokens_k, tile_tokens, group_tokens, causal, two_groups, paged;
   int max_len;  // pages: what the page table can hold
+  int packs, ctas, max_pieces, max_splits, max_parts;
 };
 
 struct SeqExtent {
@@ -93,43 +112,68 @@ __device__ __forceinline__ VarTile make_tile(const ScheduleParams& p, const SeqE
   };
   t.n0 = blocks(min(t.n_tok, p.group_tokens));
   t.n1 = p.two_groups && t.n_tok > p.group_tokens ? blocks(t.n_tok) : 0;
-  t.pad = 0;
+  t.j0 = 0;
+  t.part = -1;
+  t.part_step = t.pack = t.pad = 0;
   return t;
 }
 
-// One block. A counting sort of all tiles by their KV blocks, most first; one warp per sequence at a time. The order
-// inside a bucket is left to the atomics: it decides which CTA runs a tile, not what the tile computes.
+// One block. Cuts the tiles (below), then a counting sort of all pieces by their KV blocks, most first (a piece of one group
+// takes as long as one of two: what counts is the longer walk); one warp per sequence at a time. The order inside a bucket and the places of the parts are left to the atomics: they decide which CTA runs a
+// piece and where its part lies, not what is computed.
+//
+// A tile of n blocks is cut into ceil(n / cap) even pieces with cap = all blocks of all packs / CTAs (at least
+// VAR_MIN_BLOCKS): nothing is cut while every tile is shorter than an even share, and then at most two pieces per CTA
+// exist, which bounds the workspace: the pieces of cut tiles number at most blocks / cap + cut tiles <= 2 CTAs.
 static constexpr int SCHED_BUCKETS = 1024;
 __global__ void __launch_bounds__(1024) attention_varlen_schedule_kernel(const ScheduleParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   __shared__ int count[SCHED_BUCKETS];
   __shared__ int warp_sum[32];
-  __shared__ int most;
+  __shared__ int n_split, n_parts;
+  __shared__ unsigned long long all;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   count[threadIdx.x] = 0;
-  if (threadIdx.x == 0) most = 0;
-  __syncthreads();
-  int mine = 0;
-  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
-    const SeqExtent s = seq_extent(p, b);
-    if (s.q_len > 0) mine = max(mine, s.k_len);
+  if (threadIdx.x == 0) {
+    all = 0;
+    n_split = n_parts = 0;
   }
-  atomicMax(&most, mine);
   __syncthreads();
-  const int top = 2 * ((most + VAR_BN - 1) / VAR_BN) + 2;
-  int shift = 0;
-  while ((top >> shift) >= SCHED_BUCKETS) ++shift;
   auto each_tile = [&](auto&& f) {
     for (int b = warp; b < p.batch; b += 32) {
       const SeqExtent s = seq_extent(p, b);
       const int n = (s.q_len + p.tile_tokens - 1) / p.tile_tokens;
-      for (int i = lane; i < n; i += 32) {
-        const VarTile t = make_tile(p, s, i);
-        f(t, SCHED_BUCKETS - 1 - min((t.n0 + t.n1) >> shift, SCHED_BUCKETS - 1));
-      }
+      for (int i = lane; i < n; i += 32) f(make_tile(p, s, i));
     }
   };
-  each_tile([&](const VarTile&, int bucket) { atomicAdd(&count[bucket], 1); });
+  unsigned long long mine = 0;
+  each_tile([&](const VarTile& t) { mine += max(t.n0, t.n1); });
+#pragma unroll
+  for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  if (lane == 0 && mine) atomicAdd(&all, mine);
+  __syncthreads();
+  const int cap = (int)max((all * p.packs + p.ctas - 1) / p.ctas, (unsigned long long)VAR_MIN_BLOCKS);
+  int shift = 0;  // a piece has at most cap + 1 blocks
+  while (((cap + 1ll) >> shift) >= SCHED_BUCKETS) ++shift;
+  auto bucket_of = [&](int blocks) { return SCHED_BUCKETS - 1 - min(blocks >> shift, SCHED_BUCKETS - 1); };
+  // piece i of k: the blocks n0 i / k .. n0 (i + 1) / k, and with the last one the block that only the second group has
+  auto cut = [](const VarTile& t, int i, int k) {
+    VarTile x = t;
+    x.j0 = (int)((long long)t.n0 * i / k);
+    const int end = (int)((long long)t.n0 * (i + 1) / k);
+    x.n0 = end - x.j0;
+    if (t.n1 > 0) x.n1 = (i + 1 == k ? t.n1 : end) - x.j0;
+    return x;
+  };
+  auto pieces_of = [&](const VarTile& t) { return max((t.n0 + cap - 1) / cap, 1); };
+  each_tile([&](const VarTile& t) {
+    const int k = pieces_of(t);
+    for (int i = 0; i < k; ++i) {
+      const VarTile x = cut(t, i, k);
+      atomicAdd(&count[bucket_of(max(x.n0, x.n1))], 1);
+    }
+  });
   __syncthreads();
   // exclusive prefix sum over the 1024 buckets (thread i owns bucket i)
   const int own = count[threadIdx.x];
@@ -152,15 +196,35 @@ __global__ void __launch_bounds__(1024) attention_varlen_schedule_kernel(const S
   }
   __syncthreads();
   count[threadIdx.x] = sum - own + (warp ? warp_sum[warp - 1] : 0);
-  if (threadIdx.x == 0) *p.n_tiles = min(warp_sum[31], p.cap);
   __syncthreads();
-  each_tile([&](const VarTile& t, int bucket) {
-    const int at = atomicAdd(&count[bucket], 1);
-    if (at < p.cap) {
-      reinterpret_cast<int4*>(p.tiles + at)[0] = make_int4(t.tok0, t.n_tok, t.kv_len, t.kv_first);
-      reinterpret_cast<int4*>(p.tiles + at)[1] = make_int4(t.diag, t.n0, t.n1, 0);
+  each_tile([&](const VarTile& t) {
+    const int k = pieces_of(t);
+    int part = -1;
+    if (k > 1) {
+      part = atomicAdd(&n_parts, k * p.packs);
+      const int at = atomicAdd(&n_split, 1);
+      // offsets that overlap (no sequence may) could need more: such a tile is left out
+      if (part + k * p.packs > p.max_parts || at >= p.max_splits) part = -2;
+      if (part >= 0) *reinterpret_cast<int4*>(p.splits + at) = make_int4(t.tok0, t.n_tok, part, k);
+      else if (at < p.max_splits) *reinterpret_cast<int4*>(p.splits + at) = make_int4(t.tok0, 0, 0, k);
+    }
+    for (int i = 0; i < k; ++i) {
+      const VarTile x = cut(t, i, k);
+      const int at = atomicAdd(&count[bucket_of(max(x.n0, x.n1))], 1);
+      if (at < p.max_pieces) {
+        int4* dst = reinterpret_cast<int4*>(p.pieces + at);
+        dst[0] = make_int4(x.tok0, part == -2 ? 0 : x.n_tok, x.kv_len, x.kv_first);
+        dst[1] = make_int4(x.diag, x.n0, x.n1, x.j0);
+        dst[2] = make_int4(part >= 0 ? part + i : -1, k, 0, 0);
+      }
     }
   });
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    p.count->n_pieces = min(warp_sum[31], p.max_pieces);
+    p.count->n_split = min(n_split, p.max_splits);
+    p.count->next = p.ctas;  // a CTA's first piece is that of its own number
+  }
 }
 
 // G = query groups per CTA: 2, or 1 for head dim 256 (tiles of 64 KB, an accumulator of 256 columns).
@@ -171,29 +235,49 @@ struct VarSmem {
   static constexpr int Q_OFFSET = 0;
   static constexpr int KV_OFFSET = G * TILE_BYTES;
   static constexpr int BAR_OFFSET = KV_OFFSET + KV_STAGES * TILE_BYTES;
-  static constexpr int NUM_BARS = 4 + 2 * VAR_MAX_STAGES + 16;
+  static constexpr int NUM_BARS = 4 + 2 * VAR_MAX_STAGES + 16 + 4;
   static constexpr int TOTAL = BAR_OFFSET + NUM_BARS * 8 + 16 + 1024;
 };
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tmap, uint64_t* bar, int c0, int c1, int c2,
+__device__ __forceinline__ void mbar_init_a(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+// mbar_wait with a 32-bit shared address, all of it inline: a call would cost the softmax warps registers
+// (nap: nanoseconds of sleep between two looks, for a wait that is in no hurry)
+__device__ __forceinline__ bool var_wait(uint32_t bar, uint32_t parity, int* status, int code, uint32_t nap = 0) {
+  if (mbar_try_wait_a(bar, parity)) return true;
+  uint64_t t0 = 0;
+  uint32_t spins = 0;
+  for (;;) {
+    if (mbar_try_wait_a(bar, parity)) return true;
+    if (nap) __nanosleep(nap);
+    if (((++spins) & 0xff) == 0) {
+      if (*reinterpret_cast<volatile int*>(status) != 0) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > TB200_WAIT_TIMEOUT_NS) {
+        atomicCAS(status, 0, (code << 16) | (int)(blockIdx.x & 0xffff));
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void tma_load_3d_a(uint32_t dst, const CUtensorMap* tmap, uint32_t bar, int x, int y, int z,
+                                              uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_a(uint32_t dst, const CUtensorMap* tmap, uint32_t bar, int c0, int c1, int c2,
                                             int c3, uint64_t policy) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
       " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
-      "l"(policy)
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
       : "memory");
-}
-
-// Rounds of alternating direction through the list (see the head of the file).
-__device__ __forceinline__ int var_unit(int round) {
-  const int at = (round & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
-  return round * (int)gridDim.x + at;
-}
-__device__ __forceinline__ VarTile var_tile(const VarlenParams& p, int unit) {
-  const int4* src = reinterpret_cast<const int4*>(p.tiles + unit / p.packs);
-  const int4 a = src[0], b = src[1];
-  return VarTile{a.x, a.y, a.z, a.w, b.x, b.y, b.z, 0};
 }
 
 template <int D, bool F16, int G, bool PAGED>
@@ -208,18 +292,23 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
   constexpr uint32_t TMEM_COLS = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
-  uint64_t* q_full = bars;                       // [2]
-  uint64_t* q_empty = bars + 2;                  // [2]
-  uint64_t* kv_full = bars + 4;                  // [KV]
-  uint64_t* kv_empty = kv_full + VAR_MAX_STAGES; // [KV]
-  uint64_t* s_full = kv_empty + VAR_MAX_STAGES;  // [2] MMA -> softmax: S_g ready
-  uint64_t* p_full = s_full + 2;                 // [2][4] softmax -> MMA: 32-column chunk c of P_g written (128 arrivals)
-  uint64_t* pv_done = p_full + 8;                // [2] MMA -> softmax: last PV_g of the tile complete
-  uint64_t* o_free = pv_done + 2;                // [2] softmax -> MMA: O_g read out (128 arrivals)
-  uint64_t* v_dirty = o_free + 2;                // MMA -> warps 2, 3: the V tile ahead holds rows behind the sequence's end
-  uint64_t* v_clean = v_dirty + 1;               // warps 2, 3 -> MMA: those rows are zero
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + 1);
+  // barriers by their 32-bit shared address: one register for all of them
+  const uint32_t smem_a = smem_u32(smem);
+  const uint32_t bars = smem_a + L::BAR_OFFSET;
+  const uint32_t q_full = bars;                                // [2]
+  const uint32_t q_empty = bars + 2 * 8;                       // [2]
+  const uint32_t kv_full = bars + 4 * 8;                       // [KV]
+  const uint32_t kv_empty = kv_full + VAR_MAX_STAGES * 8;      // [KV]
+  const uint32_t s_full = kv_empty + VAR_MAX_STAGES * 8;       // [2] MMA -> softmax: S_g ready
+  const uint32_t p_full = s_full + 2 * 8;                      // [2][4] softmax -> MMA: 32-column chunk c of P_g written (128 arrivals)
+  const uint32_t pv_done = p_full + 8 * 8;                     // [2] MMA -> softmax: last PV_g of the piece complete
+  const uint32_t o_free = pv_done + 2 * 8;                     // [2] softmax -> MMA: O_g read out (128 arrivals)
+  const uint32_t v_dirty = o_free + 2 * 8;                     // MMA -> warp 2: the V tile ahead holds rows behind the sequence's end
+  const uint32_t v_clean = v_dirty + 8;                        // warp 2 -> MMA: those rows are zero
+  const uint32_t t_full = v_clean + 8;                         // [2] loader -> others: piece r is in slot r % 2
+  const uint32_t t_empty = t_full + 2 * 8;                     // [2] others -> loader: read (one arrival per warp that runs)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFFSET + (L::NUM_BARS) * 8);
+  __shared__ VarTile tile_slot[2];  // a variable of its own, so that what is read from it is known to be warp-uniform
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -229,19 +318,23 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
     tma_prefetch_desc(&p.tmk);
     tma_prefetch_desc(&p.tmv);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      for (int c = 0; c < 4; ++c) mbar_init(&p_full[i * 4 + c], 128);
-      mbar_init(&pv_done[i], 1);
-      mbar_init(&o_free[i], 128);
+      mbar_init_a(q_full + 8 * (i), 1);
+      mbar_init_a(q_empty + 8 * (i), 1);
+      mbar_init_a(s_full + 8 * (i), 1);
+      for (int c = 0; c < 4; ++c) mbar_init_a(p_full + 8 * (i * 4 + c), 128);
+      mbar_init_a(pv_done + 8 * (i), 1);
+      mbar_init_a(o_free + 8 * (i), 128);
     }
     for (int i = 0; i < VAR_MAX_STAGES; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init_a(kv_full + 8 * (i), 1);
+      mbar_init_a(kv_empty + 8 * (i), 1);
     }
-    mbar_init(v_dirty, 1);
-    mbar_init(v_clean, 2);
+    mbar_init_a(v_dirty, 1);
+    mbar_init_a(v_clean, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init_a(t_full + 8 * (i), 1);
+      mbar_init_a(t_empty + 8 * (i), 2 + 4 * G);
+    }
     mbar_init_fence();
   }
   if (warp == 1) {
@@ -254,9 +347,16 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the schedule
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   int* const status = p.status;
-  const int units = *p.n_tiles * p.packs;
-  const uint32_t smem_a = smem_u32(smem);
-  const int group_tokens = 128 >> p.lgp;
+  const int group_tokens = 128 / p.gp;
+  // The r-th piece of this CTA, for the one thread of a warp that asks.
+  auto next_tile = [&](uint32_t r, VarTile& t, uint32_t nap) -> bool {
+    if (!var_wait(t_full + 8 * (r & 1), (r >> 1) & 1, status, WAIT_ATTN, nap)) return false;
+    const int4* src = reinterpret_cast<const int4*>(tile_slot + (r & 1));
+    const int4 a = src[0], b = src[1], c = src[2];
+    t = VarTile{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, 0};
+    mbar_arrive_a(t_empty + 8 * (r & 1));
+    return t.n0 > 0;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ loader (whole warp; lane 0 waits and counts)
@@ -264,14 +364,16 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
     const uint64_t pol_q = policy_evict_first();
     const uint64_t pol_kv = policy_evict_last();
     const int n_boxes = PAGED ? VAR_BN / p.box_rows : 1;
+    const uint32_t q_bytes = (uint32_t)(group_tokens * p.gp) * (D * 2);
+    const int units = p.count->n_pieces * p.packs;
     uint32_t pos = 0, tc0 = 0, tc1 = 0;
     bool ok = true;
     auto load_q = [&](int g, const VarTile& t, int pack) {
       if (lane == 0) {
-        mbar_expect_tx(&q_full[g], L::TILE_BYTES);
+        mbar_expect_tx_a(q_full + 8 * (g), q_bytes);
 #pragma unroll
         for (int b = 0; b < DBOX; ++b)
-          tma_load_4d(smem + L::Q_OFFSET + g * L::TILE_BYTES + b * BOX_BYTES, &p.tmq, &q_full[g], b * 64, 0,
+          tma_load_4d_a(smem_a + L::Q_OFFSET + g * L::TILE_BYTES + b * BOX_BYTES, &p.tmq, q_full + 8 * g, b * 64, 0,
                       t.tok0 + g * group_tokens, pack, pol_q);
       }
     };
@@ -287,51 +389,80 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
       const uint32_t stage = pos % KV_STAGES;
       bool go = true;
       if (lane == 0) {
-        go = mbar_wait(&kv_empty[stage], ((pos / KV_STAGES) & 1) ^ 1, status, WAIT_SMEM_EMPTY);
-        if (go) mbar_expect_tx(&kv_full[stage], L::TILE_BYTES);
+        go = var_wait(kv_empty + 8 * (stage), ((pos / KV_STAGES) & 1) ^ 1, status, WAIT_SMEM_EMPTY);
+        if (go) mbar_expect_tx_a(kv_full + 8 * (stage), L::TILE_BYTES);
       }
       go = __shfl_sync(0xffffffffu, (int)go, 0) != 0;
       if (!go) return false;
-      uint8_t* dst = smem + L::KV_OFFSET + stage * L::TILE_BYTES;
+      const uint32_t dst = smem_a + L::KV_OFFSET + stage * L::TILE_BYTES;
       if (PAGED) {
         if (lane < n_boxes) {
           const int in_page = (j * VAR_BN + lane * p.box_rows) % p.page_size;
 #pragma unroll
           for (int b = 0; b < DBOX; ++b)
-            tma_load_4d(dst + b * BOX_BYTES + lane * p.box_rows * 128, tm, &kv_full[stage], b * 64, in_page, kvh, page,
+            tma_load_4d_a(dst + b * BOX_BYTES + lane * p.box_rows * 128, tm, kv_full + 8 * stage, b * 64, in_page, kvh, page,
                         pol_kv);
         }
       } else if (lane == 0) {
 #pragma unroll
         for (int b = 0; b < DBOX; ++b)
-          tma_load_3d(dst + b * BOX_BYTES, tm, &kv_full[stage], b * 64, t.kv_first + j * VAR_BN, kvh, pol_kv);
+          tma_load_3d_a(dst + b * BOX_BYTES, tm, kv_full + 8 * stage, b * 64, t.kv_first + j * VAR_BN, kvh, pol_kv);
       }
       ++pos;
       return true;
     };
     auto wait_q = [&](int g, uint32_t count) -> bool {
       bool go = true;
-      if (lane == 0) go = mbar_wait(&q_empty[g], (count & 1) ^ 1, status, WAIT_SMEM_EMPTY);
+      if (lane == 0) go = var_wait(q_empty + 8 * (g), (count & 1) ^ 1, status, WAIT_SMEM_EMPTY);
       return __shfl_sync(0xffffffffu, (int)go, 0) != 0;
     };
-    for (int r = 0; ok; ++r) {
-      const int unit = var_unit(r);
-      if (r * (int)gridDim.x >= units) break;
-      if (unit >= units) continue;
-      const VarTile t = var_tile(p, unit);
-      const int pack = unit % p.packs, kvh = pack / p.packs_per_kv;
-      const int n = max(t.n0, t.n1);
-      int page = page_of(t, 0);
+    int unit = blockIdx.x;
+    auto fetch = [&](int u) {
+      VarTile t = {};  // n0 = 0: the end
+      if (u < units) {
+        const int4* src = reinterpret_cast<const int4*>(p.pieces + u / p.packs);
+        const int4 a = src[0], b = src[1], c = src[2];
+        const int pack = u % p.packs;
+        t = VarTile{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x < 0 ? -1 : c.x + pack * c.y, c.y, pack, 0};
+      }
+      return t;
+    };
+    VarTile ahead = fetch(unit);
+    for (uint32_t r = 0; ok; ++r) {
+      const VarTile t = ahead;
+      if (lane == 0) {
+        ok = var_wait(t_empty + 8 * (r & 1), ((r >> 1) & 1) ^ 1, status, WAIT_ATTN);
+        if (ok) {
+          tile_slot[r & 1] = t;
+          mbar_arrive_a(t_full + 8 * (r & 1));
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (!ok || t.n0 == 0) break;
+      const int kvh = t.pack / p.packs_per_kv;
+      const int n = max(t.n0, t.n1), end = t.j0 + n;
+      // The next piece is drawn two blocks ahead of this one's end and looked up a block later: any later and the ring
+      // would run empty, much earlier (all second pieces at once, in whatever order the CTAs start) cost a quarter on
+      // two unequal pieces per CTA.
+      int next = 0;
+      auto draw = [&](int j) {
+        if (j == max(end - 2, t.j0) && lane == 0) next = atomicAdd(&p.count->next, 1);
+        if (j == end - 1) ahead = fetch(__shfl_sync(0xffffffffu, next, 0));
+      };
+      int page = page_of(t, t.j0), page_ahead = n > 1 ? page_of(t, t.j0 + 1) : 0;
       if (!wait_q(0, tc0++)) break;
-      load_q(0, t, pack);
-      if (!load_kv(&p.tmk, t, kvh, 0, page)) break;
+      load_q(0, t, t.pack);
+      if (!load_kv(&p.tmk, t, kvh, t.j0, page)) break;
       if (TWO && t.n1 > 0) {
         if (!wait_q(1, tc1++)) break;
-        load_q(1, t, pack);
+        load_q(1, t, t.pack);
       }
-      if (!load_kv(&p.tmv, t, kvh, 0, page)) break;
-      for (int j = 1; j < n && ok; ++j) {
-        page = page_of(t, j);
+      if (!load_kv(&p.tmv, t, kvh, t.j0, page)) break;
+      draw(t.j0);
+      for (int j = t.j0 + 1; j < end && ok; ++j) {
+        page = page_ahead;
+        if (j + 1 < end) page_ahead = page_of(t, j + 1);
+        draw(j);
         ok = load_kv(&p.tmk, t, kvh, j, page) && load_kv(&p.tmv, t, kvh, j, page);
       }
     }
@@ -360,7 +491,7 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
           const uint64_t off = (uint64_t)(((k >> 2) * BOX_BYTES + (k & 3) * 32) >> 4);
           umma_f16_ss(d_s, qd + off, kd + off, idq, k > 0 ? 1u : 0u);
         }
-        umma_commit(&s_full[g]);
+        umma_commit_a(s_full + 8 * (g));
       };
       // PV_g in four slices of 32 keys, each as soon as the softmax has published that chunk of P_g
       auto issue_pv = [&](int g, uint32_t vstage, uint32_t accum, uint32_t iph, bool ready, bool last) -> bool {
@@ -369,14 +500,14 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
         const uint32_t a_p = tmem_base + g * S_COLS;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (!ready && !mbar_wait(&p_full[g * 4 + c], iph, status, WAIT_ATTN)) return false;
+          if (!ready && !var_wait(p_full + 8 * (g * 4 + c), iph, status, WAIT_ATTN)) return false;
           tc_fence_after_sync();
-          if (c < 3) ready = mbar_test(&p_full[g * 4 + c + 1], iph);  // probe ahead of this slice's MMAs
+          if (c < 3) ready = mbar_test_a(p_full + 8 * (g * 4 + c + 1), iph);  // probe ahead of this slice's MMAs
 #pragma unroll
           for (int k = 2 * c; k < 2 * (c + 1); ++k)
             umma_f16_ts(d_o, a_p + k * 8, vd + (uint64_t)((k * 16 * 128) >> 4), idp, (k > 0) ? 1u : accum);
         }
-        if (last) umma_commit(&pv_done[g]);
+        if (last) umma_commit_a(pv_done + 8 * (g));
         return true;
       };
       auto advance = [&]() {
@@ -386,109 +517,151 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
         }
       };
 
-      for (int r = 0; ok; ++r) {
-        const int unit = var_unit(r);
-        if (r * (int)gridDim.x >= units) break;
-        if (unit >= units) continue;
-        const VarTile t = var_tile(p, unit);
+      // One stream of blocks across the pieces: the first scores of the next piece are issued where the next block's would
+      // be, between the last P V of the two groups, so they are there when a group has written its results out.
+      uint32_t r = 0;
+      VarTile t, u;
+      bool have = next_tile(r, t, 0);
+      u = t;
+      for (bool first = true; have;) {
         const int n0 = t.n0, n1 = TWO ? t.n1 : 0, n = max(n0, n1);
         const bool both = TWO && n1 > 0;
         const uint32_t tph0 = tc0++ & 1, tph1 = tc1 & 1;
         if (both) ++tc1;
-        // prologue: S_g(0) = Q_g K(0)^T
-        const uint32_t kcur = kvs, kcur_ph = kvph;
-        advance();
-        if (!mbar_wait(&q_full[0], tph0, status, WAIT_ATTN)) break;
-        if (!mbar_wait(&kv_full[kcur], kcur_ph, status, WAIT_SMEM_FULL)) break;
-        tc_fence_after_sync();
-        issue_qk(0, kcur);
-        if (both) {
-          if (!mbar_wait(&q_full[1], tph1, status, WAIT_ATTN)) break;
+        // A walk that ends behind the sequence's end: its last V tile is cleaned before use. The helper is told once the
+        // full phase before that tile's in its ring stage has been seen here, so its wait cannot mistake an earlier phase
+        // for it, and not again before it has answered.
+        const bool tail = (t.j0 + n) * VAR_BN > t.kv_len;
+        // S_g(0) = Q_g K(0)^T of piece x (its K tile in stage k): called for each group in its place
+        auto begin0 = [&](const VarTile& x, uint32_t k, uint32_t qph) -> bool {
+          if (!var_wait(q_full, qph, status, WAIT_ATTN)) return false;
           tc_fence_after_sync();
-          issue_qk(1, kcur);
+          issue_qk(0, k);
+          if (x.n0 == 1) umma_commit_a(q_empty);
+          return true;
+        };
+        auto begin1 = [&](const VarTile& x, uint32_t k, uint32_t qph) -> bool {
+          if (TWO && x.n1 > 0) {
+            if (!var_wait(q_full + 8, qph, status, WAIT_ATTN)) return false;
+            tc_fence_after_sync();
+            issue_qk(1, k);
+          }
+          umma_commit_a(kv_empty + 8 * k);
+          if (TWO && x.n1 == 1) umma_commit_a(q_empty + 8);
+          const int blocks = max(x.n0, TWO ? x.n1 : 0);
+          if (blocks == 1 && (x.j0 + 1) * VAR_BN > x.kv_len) mbar_arrive_a(v_dirty);
+          return true;
+        };
+        if (first) {
+          first = false;
+          const uint32_t k = kvs, kph = kvph;
+          advance();
+          if (!var_wait(kv_full + 8 * k, kph, status, WAIT_SMEM_FULL) || !begin0(t, k, tph0) || !begin1(t, k, tph1)) break;
         }
-        umma_commit(&kv_empty[kcur]);
-        // A walk that ends behind the sequence's end: its last V tile is cleaned before use. The helpers are told once
-        // the full phase before that tile's in its ring stage has been seen here, so their wait cannot mistake an
-        // earlier phase for it, and not again before they have answered.
-        const bool tail = n * VAR_BN > t.kv_len;
-        if (tail && n == 1) mbar_arrive(v_dirty);
         // the second group's diagonal lies at most 128 keys behind the first one's: n0 is n1 or n1 - 1
-        if (n0 == 1) umma_commit(&q_empty[0]);
-        if (both && n1 == 1) umma_commit(&q_empty[1]);
-        for (int j = 0; j < n; ++j) {
-          const uint32_t iph0 = it0 & 1, iph1 = it1 & 1;
-          const bool act0 = j < n0, more0 = j + 1 < n0, more = j + 1 < n;
+        // All blocks but the last: this loop is kept free of everything that only borders of pieces need. What its thread
+        // does between two tcgen05.mma is idle time of the tensor pipe.
+        for (int j = 0; j + 1 < n; ++j) {
+          const uint32_t iph0 = it0++ & 1, iph1 = it1 & 1;
+          const bool more0 = j + 1 < n0;
           const uint32_t vcur = kvs, vcur_ph = kvph;
           advance();
-          uint32_t knext = 0, knext_ph = 0;
-          if (more) {
-            knext = kvs;
-            knext_ph = kvph;
-            advance();
-          }
-          if (!mbar_wait(&kv_full[vcur], vcur_ph, status, WAIT_SMEM_FULL)) { ok = false; break; }
-          if (tail && j == n - 2) mbar_arrive(v_dirty);
-          if (tail && j == n - 1) {
-            if (!mbar_wait(v_clean, clean++ & 1, status, WAIT_ATTN)) { ok = false; break; }
-            tc_fence_after_sync();
-          }
-          const bool k_ready = more && mbar_test(&kv_full[knext], knext_ph);
-          if (act0) {
-            if (j == 0 && !mbar_wait(&o_free[0], tph0 ^ 1, status, WAIT_ATTN)) { ok = false; break; }
-            if (!issue_pv(0, vcur, j > 0 ? 1u : 0u, iph0, mbar_test(&p_full[0], iph0), !more0)) { ok = false; break; }
-            ++it0;
-          }
-          bool p1_ready = false;
-          if (more) {
-            if (!k_ready && !mbar_wait(&kv_full[knext], knext_ph, status, WAIT_SMEM_FULL)) { ok = false; break; }
-            tc_fence_after_sync();
-            if (both) p1_ready = mbar_test(&p_full[4], iph1);
-            if (more0) {
-              issue_qk(0, knext);
-              if (j + 2 == n0) umma_commit(&q_empty[0]);
-            }
+          const uint32_t knext = kvs, knext_ph = kvph;
+          advance();
+          if (!var_wait(kv_full + 8 * vcur, vcur_ph, status, WAIT_SMEM_FULL)) { ok = false; break; }
+          if (tail && j == n - 2) mbar_arrive_a(v_dirty);
+          const bool k_ready = mbar_test_a(kv_full + 8 * knext, knext_ph);
+          if (j == 0 && !var_wait(o_free, tph0 ^ 1, status, WAIT_ATTN)) { ok = false; break; }
+          if (!issue_pv(0, vcur, j > 0 ? 1u : 0u, iph0, mbar_test_a(p_full, iph0), !more0)) { ok = false; break; }
+          if (!k_ready && !var_wait(kv_full + 8 * knext, knext_ph, status, WAIT_SMEM_FULL)) { ok = false; break; }
+          tc_fence_after_sync();
+          const bool p1_ready = both && mbar_test_a(p_full + 8 * 4, iph1);
+          if (more0) {
+            issue_qk(0, knext);
+            if (j + 2 == n0) umma_commit_a(q_empty);
           }
           if (both) {
-            if (j == 0 && !mbar_wait(&o_free[1], tph1 ^ 1, status, WAIT_ATTN)) { ok = false; break; }
-            if (!issue_pv(1, vcur, j > 0 ? 1u : 0u, iph1, p1_ready, !more)) { ok = false; break; }
+            if (j == 0 && !var_wait(o_free + 8, tph1 ^ 1, status, WAIT_ATTN)) { ok = false; break; }
+            if (!issue_pv(1, vcur, j > 0 ? 1u : 0u, iph1, p1_ready, false)) { ok = false; break; }
             ++it1;
           }
-          umma_commit(&kv_empty[vcur]);
-          if (more) {
-            if (both) issue_qk(1, knext);
-            umma_commit(&kv_empty[knext]);
-            if (both && j + 2 == n1) umma_commit(&q_empty[1]);
-          }
+          umma_commit_a(kv_empty + 8 * vcur);
+          if (both) issue_qk(1, knext);
+          umma_commit_a(kv_empty + 8 * knext);
+          if (both && j + 2 == n1) umma_commit_a(q_empty + 8);
         }
+        if (!ok) break;
+        // the last block, with the first scores of the next piece
+        const uint32_t accum = n > 1 ? 1u : 0u;
+        const uint32_t vcur = kvs, vcur_ph = kvph;
+        advance();
+        if (!var_wait(kv_full + 8 * vcur, vcur_ph, status, WAIT_SMEM_FULL)) break;
+        if (tail) {
+          if (!var_wait(v_clean, clean++ & 1, status, WAIT_ATTN)) break;
+          tc_fence_after_sync();
+        }
+        if (n0 == n) {
+          if (n == 1 && !var_wait(o_free, tph0 ^ 1, status, WAIT_ATTN)) break;
+          if (!issue_pv(0, vcur, accum, it0++ & 1, false, true)) break;
+        }
+        have = next_tile(++r, u, 0);
+        uint32_t knext = 0;
+        if (have) {
+          knext = kvs;
+          const uint32_t knext_ph = kvph;
+          advance();
+          if (!var_wait(kv_full + 8 * knext, knext_ph, status, WAIT_SMEM_FULL)) break;
+          if (!begin0(u, knext, tc0 & 1)) break;
+        }
+        if (both) {
+          if (n == 1 && !var_wait(o_free + 8, tph1 ^ 1, status, WAIT_ATTN)) break;
+          if (!issue_pv(1, vcur, accum, it1++ & 1, false, true)) break;
+        }
+        umma_commit_a(kv_empty + 8 * vcur);
+        if (have && !begin1(u, knext, tc1 & 1)) break;
+        t = u;
       }
     }
-  } else if (warp < 4) {
+  } else if (warp == 3) {
+    reg_dealloc<104>();  // only takes part in the warpgroup-wide register release
+  } else if (warp == 2) {
     // ------------------------------------------------------------------ V rows behind the end of a sequence
     reg_dealloc<104>();
     uint32_t pos = 0, told = 0;
-    for (int r = 0;; ++r) {
-      const int unit = var_unit(r);
-      if (r * (int)gridDim.x >= units) break;
-      if (unit >= units) continue;
-      const VarTile t = var_tile(p, unit);
-      const int n = max(t.n0, t.n1);
-      if (n * VAR_BN > t.kv_len) {  // only the last block of a walk can reach behind the end
-        const uint32_t at = pos + 2 * (n - 1) + 1, stage = at % KV_STAGES;
-        if (!mbar_wait(v_dirty, told++ & 1, status, WAIT_ATTN)) break;
-        if (!mbar_wait(&kv_full[stage], (at / KV_STAGES) & 1, status, WAIT_SMEM_FULL)) break;
-        const int first = max(t.kv_len - (n - 1) * VAR_BN, 0);  // row r of a box lies in its bytes [128 r, 128 r + 128)
+    for (uint32_t r = 0;; ++r) {
+      // Waits here nap and one lane has them: polled at full rate by two warps they took a tenth from the softmax warps.
+      // The MMA warp says v_dirty a whole block ahead of its need.
+      int stage = -1, first = 0;
+      if (lane == 0) {
+        VarTile t;
+        if (next_tile(r, t, 32)) {
+          const int n = max(t.n0, t.n1);
+          const uint32_t at = pos + 2 * (n - 1) + 1;
+          pos += 2 * n;
+          stage = KV_STAGES;  // nothing to clean
+          if ((t.j0 + n) * VAR_BN > t.kv_len) {  // only the last block of a walk can reach behind the end
+            stage = at % KV_STAGES;
+            first = max(t.kv_len - (t.j0 + n - 1) * VAR_BN, 0);  // row r of a box lies in its bytes [128 r, 128 r + 128)
+            if (!var_wait(v_dirty, told++ & 1, status, WAIT_ATTN, 32) ||
+                !var_wait(kv_full + 8 * stage, (at / KV_STAGES) & 1, status, WAIT_SMEM_FULL, 20))
+              stage = -1;
+          }
+        }
+      }
+      stage = __shfl_sync(0xffffffffu, stage, 0);
+      first = __shfl_sync(0xffffffffu, first, 0);
+      if (stage < 0) break;
+      if (stage < (int)KV_STAGES) {
         const int chunks = (VAR_BN - first) * 8;
-        for (int i = (warp - 2) * 32 + lane; i < chunks * DBOX; i += 64) {
+        for (int i = lane; i < chunks * DBOX; i += 32) {
           const int box = i / chunks, c = i - box * chunks;
           *reinterpret_cast<uint4*>(smem + L::KV_OFFSET + stage * L::TILE_BYTES + box * BOX_BYTES + first * 128 + c * 16) =
               make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_clean);
+        if (lane == 0) mbar_arrive_a(v_clean);
       }
-      pos += 2 * n;
     }
   } else {
     // ------------------------------------------------------------------ softmax / correction / epilogue
@@ -496,38 +669,47 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
     const int g = (warp - 4) >> 2;
     const int q = warp & 3;
     const int row = q * 32 + lane;                       // row of the group
-    const int tok_row = g * group_tokens + (row >> p.lgp);  // token of the tile
-    const int head_row = row & ((1 << p.lgp) - 1);          // head of the pack
+    // token of the tile (behind every tile where the 128 rows are not whole tokens) and head of the pack, in one register:
+    // 128 scores and little else fit the loop below
+    const int place = (row < group_tokens * p.gp ? g * group_tokens + row / p.gp : 0x4000) | (row % p.gp) << 16;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
     const uint32_t t_s = tmem_base + lane_off + g * S_COLS;
     const uint32_t t_o = tmem_base + lane_off + O_COL0 + g * D;
     const float scale = p.scale_log2;
     uint32_t it = 0, tcount = 0;
     bool ok = true;
-    for (int r = 0; ok && (TWO || g == 0); ++r) {
-      const int unit = var_unit(r);
-      if (r * (int)gridDim.x >= units) break;
-      if (unit >= units) continue;
-      const VarTile t = var_tile(p, unit);
-      const int n = g == 0 ? t.n0 : t.n1;
-      if (n == 0) continue;
+    for (uint32_t r = 0; ok && (TWO || g == 0); ++r) {
+      // what the loop needs of the piece; the rest is read again behind it, so the slot is given back only there
+      if (!var_wait(t_full + 8 * (r & 1), (r >> 1) & 1, status, WAIT_ATTN)) break;
+      const volatile VarTile* slot = tile_slot + (r & 1);
+      if (slot->n0 == 0) break;
+      const int n = g == 0 ? slot->n0 : slot->n1;
+      auto give_back = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive_a(t_empty + 8 * (r & 1));
+      };
+      if (n == 0) {
+        give_back();
+        continue;
+      }
       float m = -INFINITY, l = 0.f;
-      const int last = p.causal ? min(t.kv_len - 1, t.diag + tok_row) : t.kv_len - 1;  // last visible key of this row
-      const int safe = p.causal ? min(t.kv_len - 1, t.diag + g * group_tokens) : t.kv_len - 1;  // ... of the group's first row
-      for (int j = 0; j < n; ++j, ++it) {
-        if (!mbar_wait(&s_full[g], it & 1, status, WAIT_ATTN)) { ok = false; break; }
+      const int kv_last = slot->kv_len - 1, diag = slot->diag;
+      // this row's last visible key, and that of the group's first row, counted from the block in hand
+      int last = (p.causal ? min(kv_last, diag + (place & 0xffff)) : kv_last) - slot->j0 * VAR_BN;
+      int safe = (p.causal ? min(kv_last, diag + g * group_tokens) : kv_last) - slot->j0 * VAR_BN;
+      for (int j = 0; j < n; ++j, ++it, last -= VAR_BN, safe -= VAR_BN) {
+        if (!var_wait(s_full + 8 * (g), it & 1, status, WAIT_ATTN)) { ok = false; break; }
         tc_fence_after_sync();
-        const int k0 = j * VAR_BN;
         uint32_t sv[128];
         tmem_ld_row32<0>(t_s, sv);
         tmem_ld_row32<32>(t_s + 32, sv);
         tmem_ld_row32<64>(t_s + 64, sv);
         tmem_ld_row32<96>(t_s + 96, sv);
         tmem_ld_wait();
-        if (k0 + VAR_BN - 1 > safe) {
+        if (VAR_BN - 1 > safe) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
-            if (k0 + i > last) sv[i] = 0xff800000u;  // -inf: contributes exp2(-inf) = 0
+            if (i > last) sv[i] = 0xff800000u;  // -inf: contributes exp2(-inf) = 0
         }
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
@@ -579,7 +761,7 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
           if (c > 0) {
             tmem_st_wait();
             tc_fence_before_sync();
-            mbar_arrive(&p_full[g * 4 + (c >> 5) - 1]);
+            mbar_arrive_a(p_full + 8 * (g * 4 + (c >> 5) - 1));
           }
           tmem_st_32x32b_x16(t_s + (c >> 1), pk);
         }
@@ -588,15 +770,42 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
         l += sum_lo + sum_hi;
         tmem_st_wait();
         tc_fence_before_sync();
-        mbar_arrive(&p_full[g * 4 + 3]);
+        mbar_arrive_a(p_full + 8 * (g * 4 + 3));
       }
       if (!ok) break;
-      if (!mbar_wait(&pv_done[g], tcount++ & 1, status, WAIT_ATTN)) break;
+      if (!var_wait(pv_done + 8 * (g), tcount++ & 1, status, WAIT_ATTN)) break;
       tc_fence_after_sync();
+      const int tok_row = place & 0xffff;
+      const bool valid = tok_row < slot->n_tok;
+      const long long token = slot->tok0 + tok_row;
+      const int head = slot->pack * p.gp + (place >> 16), part = slot->part;
+      give_back();
+      if (part >= 0) {
+        // a piece of a split tile: the accumulator as it is
+        const long long at = (long long)part * (G * 128) + g * 128 + row;
+        float* dst = p.part_o + at * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t_o + c, v);
+          tmem_ld_wait();
+          if (c + 32 == D) {
+            tc_fence_before_sync();
+            mbar_arrive_a(o_free + 8 * (g));
+          }
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c + 8 * i), "r"(v[8 * i]),
+                           "r"(v[8 * i + 1]), "r"(v[8 * i + 2]), "r"(v[8 * i + 3]), "r"(v[8 * i + 4]), "r"(v[8 * i + 5]),
+                           "r"(v[8 * i + 6]), "r"(v[8 * i + 7])
+                           : "memory");
+          }
+        }
+        if (valid) p.part_ml[at] = make_float2(m, l);
+        continue;
+      }
       const float inv_l = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no visible key: zeros; NaN stays NaN
-      const bool valid = tok_row < t.n_tok;
-      const long long token = t.tok0 + tok_row;
-      const int head = (unit % p.packs << p.lgp) + head_row;
       uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + token * p.o_stride_tok + head * p.o_stride_head;
       const bool wide_st = (reinterpret_cast<uintptr_t>(orow) & 31) == 0;
       auto store32 = [&](const uint32_t (&v)[32], int c) {
@@ -634,7 +843,7 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
             tmem_ld_32x32b_x32(t_o + c + 64, v0);
           } else {
             tc_fence_before_sync();
-            mbar_arrive(&o_free[g]);
+            mbar_arrive_a(o_free + 8 * (g));
           }
           store32(v1, c + 32);
         }
@@ -651,29 +860,94 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
   }
 }
 
+// Combines the parts of split tiles: a warp per row, block (x, y) = rows 32 y .. of the x-th (split tile, pack).
+template <int D, int G, bool F16>
+__global__ void __launch_bounds__(256) attention_varlen_join_kernel(const __grid_constant__ VarlenParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if ((int)blockIdx.x >= p.count->n_split * p.packs) return;
+  const int4 e = *reinterpret_cast<const int4*>(p.splits + blockIdx.x / p.packs);
+  const VarSplit s{e.x, e.y, e.z, e.w};
+  const int pack = blockIdx.x % p.packs, group_tokens = 128 / p.gp;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * 32 + warp; r < (int)blockIdx.y * 32 + 32; r += 8) {
+    const int row = r & 127, tok_row = (r >> 7) * group_tokens + row / p.gp;
+    if (row >= group_tokens * p.gp || tok_row >= s.n_tok) continue;
+    constexpr int ROWS = G * 128;
+    const long long first = (long long)(s.part + pack * s.n_parts) * ROWS + r;
+    float top = -INFINITY;
+    for (int i = lane; i < s.n_parts; i += 32) top = fmaxf(top, p.part_ml[first + i * ROWS].x);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    constexpr int COLS = D / 32;
+    float x[COLS] = {}, sum = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < s.n_parts; ++i) {
+      const float2 ml = p.part_ml[first + i * ROWS];
+      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      sum += f * ml.y;
+      const float* src = p.part_o + (first + i * ROWS) * D + lane * COLS;
+#pragma unroll
+      for (int c = 0; c < COLS; c += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + c);
+        x[c] += f * v.x;
+        x[c + 1] += f * v.y;
+      }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+    const long long token = s.tok0 + tok_row;
+    const int head = pack * p.gp + row % p.gp;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.o) + token * p.o_stride_tok + head * p.o_stride_head + lane * COLS;
+#pragma unroll
+    for (int c = 0; c < COLS; c += 2)
+      *reinterpret_cast<uint32_t*>(dst + c) =
+          F16 ? pack_f16x2(x[c] * inv, x[c + 1] * inv) : pack_bf16x2(x[c] * inv, x[c + 1] * inv);
+    if (p.lse && lane == 0) p.lse[token * p.heads + head] = top + log2f(sum);
+  }
+}
+
 template <int D, int G, bool PAGED>
-static int launch_varlen(const VarlenParams& p, bool f16, int grid, cudaStream_t stream) {
+static int launch_varlen(const VarlenParams& p, bool f16, int grid, int max_split, cudaStream_t stream) {
   using L = VarSmem<D, G>;
-  static_assert(L::TOTAL <= 232448, "shared memory budget");
+  static_assert(L::TOTAL + 2 * sizeof(VarTile) <= 232448, "shared memory budget");
   auto kfn = f16 ? attention_varlen_kernel<D, true, G, PAGED> : attention_varlen_kernel<D, false, G, PAGED>;
   if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
     return TB200_ERR_CUDA;
   // starts while the schedule is being made: barriers and tensor memory are set up by the time it is there
-  return cuda_err(launch_overlapped(kfn, dim3((unsigned)grid), VAR_THREADS, L::TOTAL, stream, p));
+  if (launch_overlapped(kfn, dim3((unsigned)grid), VAR_THREADS, L::TOTAL, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  if (max_split == 0) return TB200_OK;
+  return cuda_err(launch_overlapped(f16 ? attention_varlen_join_kernel<D, G, true> : attention_varlen_join_kernel<D, G, false>,
+                                    dim3((unsigned)max_split, 4 * G), 256, 0, stream, p));
 }
 
 struct VarPlan {
-  int lgp, tile_tokens, group_tokens;
-  int64_t cap;
+  int gp, packs, tile_tokens, group_tokens, ctas, max_split, max_parts;
+  int64_t max_pieces;
+  size_t off_splits, off_ml, off_o, bytes;
 };
+// gp: the largest divisor of the group that leaves at most 8 of a group's 128 rows unused (1 always does).
 static VarPlan var_plan(const tb200_attention_varlen_args* a) {
+  const int found = sm_count(), sms = found > 0 ? found : 148;  // a size can be asked for without a device
   VarPlan v;
   const int64_t group = a->heads / a->kv_heads;
-  v.lgp = 0;
-  while (v.lgp < 7 && group % (2 << v.lgp) == 0) ++v.lgp;
-  v.group_tokens = 128 >> v.lgp;
+  v.gp = (int)(group < 128 ? (group > 0 ? group : 1) : 128);
+  while (group % v.gp || 128 / v.gp * v.gp < 120) --v.gp;
+  v.packs = (int)(a->heads / v.gp);
+  v.group_tokens = 128 / v.gp;
   v.tile_tokens = (a->head_dim == 256 ? 1 : 2) * v.group_tokens;
-  v.cap = a->tokens_q / v.tile_tokens + a->batch;  // every sequence ends in at most one tile that is not full
+  const int64_t tiles = a->tokens_q / v.tile_tokens + a->batch;  // every sequence ends in at most one tile that is not full
+  // walks of at most VAR_MIN_BLOCKS blocks are never cut
+  const int64_t most_keys = a->page_size > 0 ? a->max_pages * a->page_size : a->tokens_k;
+  const bool cuts = most_keys > (int64_t)VAR_MIN_BLOCKS * VAR_BN;
+  v.max_split = cuts ? sms : 0;
+  v.max_parts = cuts ? 2 * sms : 0;
+  v.max_pieces = tiles + v.max_parts;
+  const int64_t units = v.max_pieces * v.packs;
+  v.ctas = (int)(units < sms ? (units > 0 ? units : 1) : sms);
+  v.off_splits = 32 + (size_t)v.max_pieces * sizeof(VarTile);
+  v.off_ml = (v.off_splits + (size_t)v.max_split * sizeof(VarSplit) + 31) / 32 * 32;
+  const size_t part_rows = (size_t)v.max_parts * (a->head_dim == 256 ? 128 : 256);
+  v.off_o = v.off_ml + part_rows * sizeof(float2);
+  v.bytes = v.off_o + part_rows * a->head_dim * sizeof(float);
   return v;
 }
 static bool var_sizes_ok(const tb200_attention_varlen_args* a) {
@@ -687,7 +961,7 @@ using namespace tb200;
 
 extern "C" size_t tb200_attention_varlen_workspace_bytes(const tb200_attention_varlen_args* a) {
   if (!var_sizes_ok(a)) return 0;
-  return 32 + (size_t)var_plan(a).cap * sizeof(VarTile);
+  return var_plan(a).bytes;
 }
 
 extern "C" int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* a, void* stream_) {
@@ -715,14 +989,10 @@ extern "C" int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* a, 
   for (const void* b : bases)
     if (reinterpret_cast<uintptr_t>(b) & 15) return TB200_ERR_BAD_ARG;
   const VarPlan plan = var_plan(a);
-  const int packs = (int)(a->heads >> plan.lgp);
-  if (plan.cap * packs > INT32_MAX / 2) return TB200_ERR_UNSUPPORTED;
-  if (!a->workspace || a->workspace_bytes < tb200_attention_varlen_workspace_bytes(a) ||
-      (reinterpret_cast<uintptr_t>(a->workspace) & 31))
+  if (plan.max_pieces * plan.packs > INT32_MAX / 2) return TB200_ERR_UNSUPPORTED;
+  if (!a->workspace || a->workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a->workspace) & 31))
     return TB200_ERR_BAD_ARG;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const int sms = sm_count();
-  if (sms <= 0) return TB200_ERR_CUDA;
 
   VarlenParams p;
   memset(&p, 0, sizeof(p));
@@ -730,8 +1000,8 @@ extern "C" int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* a, 
   const bool f16 = a->dtype == TB200_F16;
   const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   {
-    const uint64_t gp = 1ull << plan.lgp;
-    const uint64_t dims[4] = {(uint64_t)D, gp, (uint64_t)a->tokens_q, (uint64_t)packs};
+    const uint64_t gp = plan.gp;
+    const uint64_t dims[4] = {(uint64_t)D, gp, (uint64_t)a->tokens_q, (uint64_t)plan.packs};
     const uint64_t str[3] = {(uint64_t)a->q_stride_head * 2, (uint64_t)a->q_stride_tok * 2, gp * a->q_stride_head * 2};
     const uint32_t box[4] = {64, (uint32_t)gp, (uint32_t)plan.group_tokens, 1};
     const int rc = encode_tmap(&p.tmq, dt, 4, a->q, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -762,18 +1032,22 @@ extern "C" int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* a, 
   p.lse = a->lse;
   p.status = status_ptr();
   if (!p.status) return TB200_ERR_CUDA;
-  int* n_tiles = static_cast<int*>(a->workspace);
-  VarTile* tiles = reinterpret_cast<VarTile*>(static_cast<uint8_t*>(a->workspace) + 32);
-  p.tiles = tiles;
-  p.n_tiles = n_tiles;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  VarTile* pieces = reinterpret_cast<VarTile*>(ws + 32);
+  VarSplit* splits = reinterpret_cast<VarSplit*>(ws + plan.off_splits);
+  p.count = reinterpret_cast<VarCounters*>(ws);
+  p.pieces = pieces;
+  p.splits = splits;
+  p.part_ml = reinterpret_cast<float2*>(ws + plan.off_ml);
+  p.part_o = reinterpret_cast<float*>(ws + plan.off_o);
   p.page_table = a->page_table;
   p.table_stride = a->table_stride;
   p.o_stride_tok = a->o_stride_tok;
   p.o_stride_head = a->o_stride_head;
   p.heads = (int)a->heads;
-  p.packs = packs;
-  p.lgp = plan.lgp;
-  p.packs_per_kv = packs / (int)a->kv_heads;
+  p.packs = plan.packs;
+  p.gp = plan.gp;
+  p.packs_per_kv = plan.packs / (int)a->kv_heads;
   p.page_size = a->page_size;
   p.box_rows = box_rows;
   p.n_pages = (int)a->n_pages;
@@ -787,26 +1061,27 @@ extern "C" int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* a, 
   s.cu_q = a->cu_seqlens_q;
   s.cu_k = a->cu_seqlens_k;
   s.seq_lens = a->seq_lens;
-  s.tiles = tiles;
-  s.n_tiles = n_tiles;
+  s.pieces = pieces;
+  s.splits = splits;
+  s.count = p.count;
   s.batch = (int)a->batch;
   s.tokens_q = (int)a->tokens_q;
   s.tokens_k = (int)a->tokens_k;
-  s.cap = (int)plan.cap;
+  s.packs = plan.packs;
+  s.ctas = plan.ctas;
+  s.max_pieces = (int)plan.max_pieces;
+  s.max_splits = plan.max_split;
+  s.max_parts = plan.max_parts;
   s.tile_tokens = plan.tile_tokens;
   s.group_tokens = plan.group_tokens;
   s.causal = p.causal;
   s.two_groups = D == 256 ? 0 : 1;
   s.paged = paged ? 1 : 0;
   s.max_len = (int)(a->max_pages * a->page_size);
-  attention_varlen_schedule_kernel<<<1, 1024, 0, stream>>>(s);
-  if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
-
-  const int64_t most = plan.cap * packs;
-  const int grid = most < sms ? (int)most : sms;
-  if (paged)
-    return D == 256 ? launch_varlen<256, 1, true>(p, f16, grid, stream)
-           : D == 128 ? launch_varlen<128, 2, true>(p, f16, grid, stream) : launch_varlen<64, 2, true>(p, f16, grid, stream);
-  return D == 256 ? launch_varlen<256, 1, false>(p, f16, grid, stream)
-         : D == 128 ? launch_varlen<128, 2, false>(p, f16, grid, stream) : launch_varlen<64, 2, false>(p, f16, grid, stream);
+  if (launch_overlapped(attention_varlen_schedule_kernel, dim3(1), 1024, 0, stream, s) != cudaSuccess) return TB200_ERR_CUDA;
+  auto launch = paged ? (D == 256   ? launch_varlen<256, 1, true>
+                         : D == 128 ? launch_varlen<128, 2, true> : launch_varlen<64, 2, true>)
+                      : (D == 256   ? launch_varlen<256, 1, false>
+                         : D == 128 ? launch_varlen<128, 2, false> : launch_varlen<64, 2, false>);
+  return launch(p, f16, plan.ctas, plan.max_split, stream);
 }
