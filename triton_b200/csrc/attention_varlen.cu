@@ -20,6 +20,7 @@
 //   half      A tile whose tokens fit the first group (short sequences, ends) leaves the second group out.
 //   pages     A KV block is 128 / r boxes of r = gcd(page size, 128) rows; the lanes of the load warp look up and issue one
 //             page each. A page outside the pool is loaded from behind its end, which reads as zeros.
+#include <limits.h>
 #include <string.h>
 
 #include "attention_common.cuh"
@@ -147,26 +148,31 @@ __global__ void __launch_bounds__(1024) attention_varlen_schedule_kernel(const S
       for (int i = lane; i < n; i += 32) f(make_tile(p, s, i));
     }
   };
-  unsigned long long mine = 0;
-  each_tile([&](const VarTile& t) { mine += max(t.n0, t.n1); });
+  if (p.max_parts > 0) {
+    unsigned long long mine = 0;
+    each_tile([&](const VarTile& t) { mine += max(t.n0, t.n1); });
 #pragma unroll
-  for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0 && mine) atomicAdd(&all, mine);
-  __syncthreads();
-  const int cap = (int)max((all * p.packs + p.ctas - 1) / p.ctas, (unsigned long long)VAR_MIN_BLOCKS);
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0 && mine) atomicAdd(&all, mine);
+    __syncthreads();
+  }
+  const unsigned long long work = all * p.packs;
+  const int cap = max(work <= INT_MAX ? (int)work / p.ctas + 1 : (int)(work / p.ctas) + 1, VAR_MIN_BLOCKS);
   int shift = 0;  // a piece has at most cap + 1 blocks
   while (((cap + 1ll) >> shift) >= SCHED_BUCKETS) ++shift;
   auto bucket_of = [&](int blocks) { return SCHED_BUCKETS - 1 - min(blocks >> shift, SCHED_BUCKETS - 1); };
-  // piece i of k: the blocks n0 i / k .. n0 (i + 1) / k, and with the last one the block that only the second group has
+  // piece i of k even ones, the longer ones first; the last one also has the block that only the second group has
   auto cut = [](const VarTile& t, int i, int k) {
+    if (k == 1) return t;
     VarTile x = t;
-    x.j0 = (int)((long long)t.n0 * i / k);
-    const int end = (int)((long long)t.n0 * (i + 1) / k);
+    const int even = t.n0 / k, more = t.n0 - even * k;
+    x.j0 = i * even + min(i, more);
+    const int end = x.j0 + even + (i < more ? 1 : 0);
     x.n0 = end - x.j0;
     if (t.n1 > 0) x.n1 = (i + 1 == k ? t.n1 : end) - x.j0;
     return x;
   };
-  auto pieces_of = [&](const VarTile& t) { return max((t.n0 + cap - 1) / cap, 1); };
+  auto pieces_of = [&](const VarTile& t) { return t.n0 <= cap ? 1 : (t.n0 + cap - 1) / cap; };
   each_tile([&](const VarTile& t) {
     const int k = pieces_of(t);
     for (int i = 0; i < k; ++i) {
@@ -652,12 +658,10 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
       first = __shfl_sync(0xffffffffu, first, 0);
       if (stage < 0) break;
       if (stage < (int)KV_STAGES) {
-        const int chunks = (VAR_BN - first) * 8;
-        for (int i = lane; i < chunks * DBOX; i += 32) {
-          const int box = i / chunks, c = i - box * chunks;
-          *reinterpret_cast<uint4*>(smem + L::KV_OFFSET + stage * L::TILE_BYTES + box * BOX_BYTES + first * 128 + c * 16) =
-              make_uint4(0, 0, 0, 0);
-        }
+        uint8_t* rows = smem + L::KV_OFFSET + stage * L::TILE_BYTES;
+        for (int at = first * 128 + lane * 16; at < BOX_BYTES; at += 512)
+#pragma unroll
+          for (int box = 0; box < DBOX; ++box) *reinterpret_cast<uint4*>(rows + box * BOX_BYTES + at) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_a(v_clean);
