@@ -499,19 +499,28 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
         }
         umma_commit_a(s_full + 8 * (g));
       };
-      // PV_g in four slices of 32 keys, each as soon as the softmax has published that chunk of P_g
+      // PV_g at once when all of P_g is there (`ready`: its last chunk was seen; a thread arrives on the chunk barriers in
+      // order), else in four slices of 32 keys, each as soon as the softmax has published that chunk. In steady state the
+      // tensor pipe is the slower side and P_g waits for it: the waits and fences between slices of two MMAs then only
+      // left it idle.
       auto issue_pv = [&](int g, uint32_t vstage, uint32_t accum, uint32_t iph, bool ready, bool last) -> bool {
         const uint64_t vd = vdesc0 + (uint64_t)((vstage * L::TILE_BYTES) >> 4);
         const uint32_t d_o = tmem_base + O_COL0 + g * D;
         const uint32_t a_p = tmem_base + g * S_COLS;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (!ready && !var_wait(p_full + 8 * (g * 4 + c), iph, status, WAIT_ATTN)) return false;
+        if (ready) {
           tc_fence_after_sync();
-          if (c < 3) ready = mbar_test_a(p_full + 8 * (g * 4 + c + 1), iph);  // probe ahead of this slice's MMAs
 #pragma unroll
-          for (int k = 2 * c; k < 2 * (c + 1); ++k)
+          for (int k = 0; k < 8; ++k)
             umma_f16_ts(d_o, a_p + k * 8, vd + (uint64_t)((k * 16 * 128) >> 4), idp, (k > 0) ? 1u : accum);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (!var_wait(p_full + 8 * (g * 4 + c), iph, status, WAIT_ATTN)) return false;
+            tc_fence_after_sync();
+#pragma unroll
+            for (int k = 2 * c; k < 2 * (c + 1); ++k)
+              umma_f16_ts(d_o, a_p + k * 8, vd + (uint64_t)((k * 16 * 128) >> 4), idp, (k > 0) ? 1u : accum);
+          }
         }
         if (last) umma_commit_a(pv_done + 8 * (g));
         return true;
@@ -578,10 +587,10 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
           if (tail && j == n - 2) mbar_arrive_a(v_dirty);
           const bool k_ready = mbar_test_a(kv_full + 8 * knext, knext_ph);
           if (j == 0 && !var_wait(o_free, tph0 ^ 1, status, WAIT_ATTN)) { ok = false; break; }
-          if (!issue_pv(0, vcur, j > 0 ? 1u : 0u, iph0, mbar_test_a(p_full, iph0), !more0)) { ok = false; break; }
+          if (!issue_pv(0, vcur, j > 0 ? 1u : 0u, iph0, mbar_test_a(p_full + 8 * 3, iph0), !more0)) { ok = false; break; }
           if (!k_ready && !var_wait(kv_full + 8 * knext, knext_ph, status, WAIT_SMEM_FULL)) { ok = false; break; }
           tc_fence_after_sync();
-          const bool p1_ready = both && mbar_test_a(p_full + 8 * 4, iph1);
+          const bool p1_ready = both && mbar_test_a(p_full + 8 * 7, iph1);
           if (more0) {
             issue_qk(0, knext);
             if (j + 2 == n0) umma_commit_a(q_empty);
