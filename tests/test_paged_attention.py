@@ -469,6 +469,97 @@ def test_varlen_paged(cuda, causal, page, layout, d, dtype, heads, kv_heads):
 
 
 @gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,dtype,heads,kv_heads", [(128, BF16, 8, 2), (64, F16, 3, 1), (256, BF16, 4, 2), (128, F16, 12, 1)])
+@pytest.mark.parametrize("q_lens,k_lens", [([5], [9000]), ([1, 300, 2], [7000, 300, 1]), ([40, 0, 260], [3000, 4000, 2900]),
+                                           ([130] * 3, [2177] * 3), ([700], [700])])
+def test_varlen_split_walks(cuda, causal, d, dtype, heads, kv_heads, q_lens, k_lens):
+    """Few queries over many keys: walks are cut and joined, packed and over pages; the same bits every time. float16 keys of
+    a long sequence: the sum over subnormal probabilities is part of the bound."""
+    q, k, v = varlen_inputs(cuda, sum(q_lens), sum(k_lens), heads, kv_heads, d, dtype)
+    cu_q, cu_k = offsets(q_lens, cuda), offsets(k_lens, cuda)
+    o, lse = fa().attention_varlen_with_lse(q, k, v, cu_q, cu_k, 1 / math.sqrt(d), causal)
+    check_varlen(q, k, v, q_lens, k_lens, 1 / math.sqrt(d), causal, o, lse)
+    for _ in range(5):
+        again = fa().attention_varlen(q, k, v, cu_q, cu_k, 1 / math.sqrt(d), causal)
+        assert torch.equal(again.view(torch.int16), o.view(torch.int16))
+    cache = Cache(cuda, k_lens, kv_heads, d, dtype, 16)
+    fa().append_paged_kv(None, k, v, cache.k, cache.v, cache.table, cache.seq_lens, cu_k)
+    paged = fa().attention_varlen_paged(q, cache.k, cache.v, cu_q, cache.table, cache.seq_lens, 1 / math.sqrt(d), causal)
+    assert torch.equal(paged.view(torch.int16), o.view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("units", [147, 148, 149, 297])
+def test_varlen_as_many_parts_as_there_can_be(cuda, units):
+    """Equal walks just longer than an even share: every tile is cut, the parts fill the workspace."""
+    q_lens, k_lens = [1] * units, [640 + 128 * (i % 2) for i in range(units)]
+    q, k, v = varlen_inputs(cuda, units, sum(k_lens), 1, 1, 64, BF16)
+    o, lse = fa().attention_varlen_with_lse(q, k, v, offsets(q_lens, cuda), offsets(k_lens, cuda), 0.125, True)
+    check_varlen(q, k, v, q_lens, k_lens, 0.125, True, o, lse)
+
+
+@gpu
+def test_offsets_that_are_no_offsets(cuda):
+    """Offsets that run backwards, overlap or leave the tensors are wrong calls that nothing on the host can see: whatever
+    comes out, nothing outside the tensors is touched and the next call is right."""
+    q, k, v = varlen_inputs(cuda, 300, 300, 4, 2, 64, BF16)
+    cache = Cache(cuda, [300] * 3, 2, 64, BF16, 16).fill()
+    good = offsets([100, 50, 150], cuda)
+    want = fa().attention_varlen(q, k, v, good, good, 0.1, True)
+    guard = torch.full((400, 4, 64), 6.0, dtype=BF16, device=cuda)
+    for bad in ([0, 200, 100, 300], [0, 300, 0, 300], [-50, 100, 200, 4000], [2**31 - 1, -2**31, 5, 7], [300, 200, 100, 0]):
+        cu = torch.tensor(bad, dtype=torch.int32, device=cuda)
+        fa().attention_varlen(q, k, v, cu, cu, 0.1, True, out=guard[50:350])
+        fa().attention_varlen(q, k, v, good, cu, 0.1, False, out=guard[50:350])
+        fa().attention_varlen_paged(q, cache.k, cache.v, cu, cache.table, cu[:3].contiguous(), 0.1, True, out=guard[50:350])
+        fa().attention_decode(q[:3], cache.k, cache.v, cache.table, cu[:3].contiguous(), 0.1)
+        before = cache.k.clone()
+        fa().append_paged_kv(q, k, v, cache.k, cache.v, cache.table, cu[:3].contiguous(), cu, q_out=guard[50:350])
+        cache.k.copy_(before)
+        assert (guard[:50] == 6).all() and (guard[350:] == 6).all()
+    assert torch.equal(fa().attention_varlen(q, k, v, good, good, 0.1, True).view(torch.int16), want.view(torch.int16))
+
+
+@gpu
+def test_pools_of_different_order(cuda):
+    """Keys stored token by token, values head by head, and both in one tensor: the strides of the two pools are their own."""
+    cache = Cache(cuda, [130, 17, 64], 2, 128, BF16, 16).fill()
+    both = torch.full((cache.k.shape[0], 2, 16, 3, 128), math.nan, dtype=BF16, device=cuda)
+    both[:, 0, :, :2], both[:, 1, :, 1:] = cache.k, cache.v
+    head = cache.v.transpose(1, 2).contiguous().transpose(1, 2)
+    g = torch.Generator(device=cuda).manual_seed(20)
+    q = torch.randn(3, 8, 128, generator=g, device=cuda).to(BF16)
+    cu = offsets([1, 1, 1], cuda)
+    want = fa().attention_decode(q, cache.k, cache.v, cache.table, cache.seq_lens, 0.1)
+    want2 = fa().attention_varlen_paged(q, cache.k, cache.v, cu, cache.table, cache.seq_lens, 0.1, True)
+    for kk, vv in ((cache.k, head), (both[:, 0, :, :2], both[:, 1, :, 1:])):
+        got = fa().attention_decode(q, kk, vv, cache.table, cache.seq_lens, 0.1)
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+        got = fa().attention_varlen_paged(q, kk, vv, cu, cache.table, cache.seq_lens, 0.1, True)
+        assert torch.equal(got.view(torch.int16), want2.view(torch.int16))
+        new = torch.randn(3, 2, 128, generator=g, device=cuda).to(BF16)
+        fa().append_paged_kv(None, new, -new, kk, vv, cache.table, cache.seq_lens)
+        for i, n in enumerate(cache.lens):
+            page, at = int(cache.table[i, (n - 1) // 16]), (n - 1) % 16
+            assert torch.equal(kk[page, at], new[i]) and torch.equal(vv[page, at], -new[i])
+        kk.copy_(cache.k) if kk is not cache.k else kk.copy_(both[:, 0, :, :2])
+    assert both[:, 0, :, 2].isnan().all() and both[:, 1, :, 0].isnan().all()
+
+
+@gpu
+def test_decode_same_bits_every_time(cuda):
+    for lens, heads, kv in (([9000], 8, 1), ([700] * 70, 8, 2), ([0, 5, 3000, 1], 24, 2)):
+        cache = Cache(cuda, lens, kv, 128, BF16, 16).fill()
+        g = torch.Generator(device=cuda).manual_seed(21)
+        q = torch.randn(len(lens), heads, 128, generator=g, device=cuda).to(BF16)
+        want, lse = fa().attention_decode_with_lse(q, cache.k, cache.v, cache.table, cache.seq_lens, 0.1)
+        for _ in range(10):
+            got, lse2 = fa().attention_decode_with_lse(q, cache.k, cache.v, cache.table, cache.seq_lens, 0.1)
+            assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and torch.equal(lse, lse2)
+
+
+@gpu
 def test_varlen_paged_missing_pages(cuda):
     cache = Cache(cuda, [300, 200], 2, 128, BF16, 16).fill()
     cache.table[0, 3], cache.table[0, 18], cache.table[1, 0] = -1, 1 << 30, cache.k.shape[0]

@@ -86,15 +86,15 @@ struct SeqExtent {
   int q0, q_len, k_len, k_first;
 };
 __device__ __forceinline__ SeqExtent seq_extent(const ScheduleParams& p, int b) {
-  SeqExtent s;
-  s.q0 = max(p.cu_q[b], 0);
-  s.q_len = max(min(p.cu_q[b + 1], p.tokens_q) - s.q0, 0);
+  SeqExtent s;  // every offset is brought into its tensor before it is used: a wrong one costs results, not memory
+  s.q0 = min(max(p.cu_q[b], 0), p.tokens_q);
+  s.q_len = max(min(max(p.cu_q[b + 1], 0), p.tokens_q) - s.q0, 0);
   if (p.paged) {
     s.k_len = min(max(p.seq_lens[b], 0), p.max_len);
     s.k_first = b;
   } else {
     s.k_first = min(max(p.cu_k[b], 0), p.tokens_k);
-    s.k_len = max(min(p.cu_k[b + 1], p.tokens_k) - s.k_first, 0);
+    s.k_len = max(min(max(p.cu_k[b + 1], 0), p.tokens_k) - s.k_first, 0);
     if (s.k_len == 0) s.k_first = max(p.tokens_k, 1);  // behind the last row: the one block loaded for it is all zeros
   }
   return s;

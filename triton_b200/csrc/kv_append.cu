@@ -109,16 +109,17 @@ __global__ void __launch_bounds__(APP_WARPS * 32) kv_append_kernel(const __grid_
   }
 
   // ---- the token's sequence, position, table row and page
-  int b = (int)t, pos;
+  int b = (int)t;
+  long long at = 1;  // rows from this one to the end of its sequence
   if (a.cu_seqlens) {
     b = find_sequence(a.cu_seqlens, (int)a.batch, (int)t, lane);
     if (b < 0) return;
     const int end = a.cu_seqlens[b + 1];
     if ((int)t >= end) return;  // behind the last sequence
-    pos = a.seq_lens[b] - (end - (int)t);
-  } else {
-    pos = a.seq_lens[b] - 1;
+    at = (long long)end - t;
   }
+  const long long position = a.seq_lens[b] - at;
+  const int pos = position >= 0 ? (int)position : -1;
   const int slot = pos >= 0 ? pos / a.page_size : -1;
   const bool valid = pos >= 0 && slot < a.max_pages && (!a.cos || pos < a.n_positions);
   int64_t page = -1;

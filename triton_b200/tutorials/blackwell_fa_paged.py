@@ -157,13 +157,15 @@ def _ptr(t):
 
 def _call(name, args, idx, rows=None):
     """Launches on the current stream of the data's device; `rows`: any tensor there, to allocate the call's workspace from."""
+    if torch._C._cuda_getDevice() != idx:
+        with torch.cuda.device(idx):
+            return _call(name, args, idx, rows)
     lib, ref = _lib.lib(), ctypes.byref(args)
-    with _lib.device_guard(idx):
-        if rows is not None:
-            need = getattr(lib, name[0])(ref)
-            ws = rows.new_empty(need // 2 + 1)
-            args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        rc = getattr(lib, name[-1])(ref, _lib.current_stream_ptr(idx))
+    if rows is not None:
+        need = getattr(lib, name[0])(ref)
+        ws = rows.new_empty(need // 2 + 1)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    rc = getattr(lib, name[-1])(ref, _lib.current_stream_ptr(idx))
     if rc:
         _lib.check(rc, name[-1])
 
