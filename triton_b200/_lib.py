@@ -6,6 +6,7 @@ raise. ``lib()`` loads the library on first use.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -218,6 +219,16 @@ class Mxfp4UpcastArgs(Structure):
         ("w", c_void_p), ("w_scale", c_void_p), ("out", c_void_p),
         ("n_experts", c_int64), ("k", c_int64), ("n", c_int64), ("out_dtype", c_int32),
     ]
+
+
+_FORMAT = {c_void_p: "Q", c_size_t: "Q", c_int64: "q", c_int32: "i", c_float: "f"}
+
+
+def packed(cls):
+    """A constructor of `cls` from all of its fields in order (null pointers as 0), about three times as fast as the class
+    itself: for the calls of a decode step, whose kernels take a few microseconds."""
+    pack, copy = struct.Struct("@" + "".join(_FORMAT[t] for _, t in cls._fields_)).pack, cls.from_buffer_copy
+    return lambda *fields: copy(pack(*fields))
 
 
 _lib = None

@@ -38,6 +38,7 @@ from .. import _lib
 
 _DT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _HEAD_DIMS = (64, 128, 256)
+_append_args, _decode_args, _varlen_args = map(_lib.packed, (_lib.KvAppendArgs, _lib.AttentionDecodeArgs, _lib.AttentionVarlenArgs))
 
 
 # The checks below run on every call of a decode step, whose kernels take a few microseconds: each tensor's shape and strides
@@ -152,7 +153,7 @@ def _aligned(t):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _call(name, args, idx, rows=None):
@@ -215,7 +216,7 @@ def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=
     q, qs, qh = (None, 0, 0) if q is None else _in_rows(q)
     k, ks, kh = _in_rows(k)
     v, vs, vh = _in_rows(v)
-    args = _lib.KvAppendArgs(
+    args = _append_args(
         _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(qo), _ptr(ko), k_cache.data_ptr(), v_cache.data_ptr(),
         page_table.data_ptr(), seq_lens.data_ptr(), _ptr(cu_seqlens), _ptr(cos), _ptr(sin), _ptr(k_scale), _ptr(v_scale),
         tokens, batch, 0 if q is None else heads, kv_heads, qs, qh, ks, kh, vs, vh, qos, qoh, kos, koh, *kst, *vst,
@@ -237,10 +238,10 @@ def _decode(q, k_cache, v_cache, page_table, seq_lens, sm_scale, k_scale, v_scal
     o, os, oh = _out_rows(out, q, "out")
     q, qs, qh = _in_rows(q)
     lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if with_lse else None
-    args = _lib.AttentionDecodeArgs(
+    args = _decode_args(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _ptr(lse), page_table.data_ptr(),
-        seq_lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), None, 0, batch, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
-        table_stride, n_pages, max_pages, page_size, d, _DT[dtype], cache_dt, kn, vn, float(sm_scale))
+        seq_lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), 0, 0, batch, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
+        table_stride, n_pages, max_pages, page_size, d, _DT[dtype], cache_dt, kn, vn, float(sm_scale), 0)
     _call(("tb200_attention_decode_workspace_bytes", "tb200_attention_decode"), args, idx, q)
     return o, lse
 
@@ -262,10 +263,10 @@ def _varlen(what, q, k, v, kst, vst, cu_q, cu_k, page_table, seq_lens, tokens_k,
     o, os, oh = _out_rows(out, q, "out")
     q, qs, qh = _in_rows(q)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if with_lse else None
-    args = _lib.AttentionVarlenArgs(
+    args = _varlen_args(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), cu_q.data_ptr(), _ptr(cu_k), _ptr(page_table),
-        _ptr(seq_lens), None, 0, tokens, tokens_k, cu_q.shape[0] - 1, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
-        table_stride, n_pages, max_pages, page_size, d, _DT[q.dtype], 1 if causal else 0, float(sm_scale))
+        _ptr(seq_lens), 0, 0, tokens, tokens_k, cu_q.shape[0] - 1, heads, kv_heads, qs, qh, os, oh, *kst, *vst,
+        table_stride, n_pages, max_pages, page_size, d, _DT[q.dtype], 1 if causal else 0, float(sm_scale), 0)
     _call(("tb200_attention_varlen_workspace_bytes", "tb200_attention_varlen_fwd"), args, idx, q)
     return o, lse
 
