@@ -166,7 +166,7 @@ def _call(name, args, idx, rows=None):
         need = getattr(lib, name[0])(ref)
         ws = rows.new_empty(need // 2 + 1)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    rc = getattr(lib, name[-1])(ref, _lib.current_stream_ptr(idx))
+    rc = getattr(lib, name[-1])(ref, torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         _lib.check(rc, name[-1])
 
