@@ -284,6 +284,32 @@ def test_decode_long_and_many(cuda, batch, length, cache_dtype):
 
 
 @gpu
+@pytest.mark.parametrize("batch", [127, 128, 129, 300, 1500])
+def test_many_sequences(cuda, batch):
+    """More sequences than threads of a block, than 32 and than 1024 probes of a search; some of them empty."""
+    g = torch.Generator(device=cuda).manual_seed(22)
+    past = [(i * 7) % 40 if i % 5 else 0 for i in range(batch)]
+    new = [(i * 3) % 4 for i in range(batch)]
+    lens = [p + n for p, n in zip(past, new)]
+    cache = Cache(cuda, lens, 1, 64, BF16, 8).fill()
+    q, k, v = append_inputs(cuda, sum(new), 2, 1, 64, BF16)
+    before = cache.k.clone(), cache.v.clone()
+    q_out = fa().append_paged_kv(q, k, v, cache.k, cache.v, cache.table, cache.seq_lens, offsets(new, cuda))
+    seq_of = torch.repeat_interleave(torch.arange(batch), torch.tensor(new)).to(cuda)
+    positions = torch.cat([torch.arange(p, p + n) for p, n in zip(past, new)]).to(cuda)
+    check_append(cache, q, k, v, q_out, None, positions, seq_of, None, None, False, before)
+    check_decode(cache, torch.randn(batch, 2, 64, generator=g, device=cuda).to(BF16), 0.125)
+    o, lse = fa().attention_varlen_paged_with_lse(q, cache.k, cache.v, offsets(new, cuda), cache.table, cache.seq_lens, 0.125, True)
+    at = 0
+    for i, n in enumerate(new):
+        kk, vv = cache.rows(i)
+        want, row, size = ref.sequence_attention(q[at:at + n].double(), kk, vv, 0.125, True)
+        check_attention(o[at:at + n], want, size, BF16, lens[i], 1.0)
+        check_lse(lse[at:at + n], row)
+        at += n
+
+
+@gpu
 def test_decode_scores_that_grow_and_large_scores(cuda):
     """The running maximum moves by far more than the accumulator's headroom, up along one sequence and down along another;
     the largest scores are near 2^9, where a 32-bit score is off by up to 2^9 * 2^-24 * 128 = 2^-8 in the exponent."""

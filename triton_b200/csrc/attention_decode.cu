@@ -11,6 +11,9 @@
 // zeros without an access). The products run on the tensor cores with the keys as the long side: S^T [16 keys, 8 heads] =
 // K Q^T and O^T [16 columns, 8 heads] += V^T P^T by mma.m16n8k16, so a group of up to 8 heads fills the 8-wide side whatever
 // its size. tcgen05 has no use here: its 128-row tile would be filled by 8 heads, and the kernel is bound by reading K and V.
+// Bound: HBM. 2 sequences of 374000 tokens, 64 / 8 heads of 128 in bf16: 459 us = 6.7 TB/s; 64 sequences of 9000 in e4m3:
+// 199 us = 6.0 TB/s; 48 sequences up to 6000 tokens, 32 / 8 heads: 45 us, of which 23 are reading and the rest start-up,
+// merging and joining.
 // e4m3 pools are widened to float16 in registers (exact); queries are then brought to [1, 2) by a power of two per head
 // first, so that they fit. P is rounded to the type of V (float16 for e4m3), everything else is kept in 32 bits.
 #include <cuda_bf16.h>
