@@ -66,9 +66,10 @@ struct DecCfg {
   static constexpr int LIMIT = 233472 / CTAS - 1024;
   // A part that is cut at a piece's end takes the place of the warp's ring, which is empty by then; one that is cut at its
   // start has shared memory of its own where that fits, else it goes through the workspace.
-  static constexpr bool HEAD_SMEM = RING + DEC_WARPS * HEAD + PARTS * (NH * 8 + 16) + 128 <= LIMIT;
+  static constexpr int SCRATCH = DEC_WARPS * (2 * 4 + 16);  // of the kernel's head: sums and starts of its warps
+  static constexpr bool HEAD_SMEM = RING + DEC_WARPS * HEAD + PARTS * (NH * 8 + 16) + SCRATCH <= LIMIT;
   static constexpr int HEADS = HEAD_SMEM ? DEC_WARPS * HEAD : 0;
-  static constexpr int SMEM = RING + HEADS + PARTS * (NH * 8 + 16) + 128;
+  static constexpr int SMEM = RING + HEADS + PARTS * (NH * 8 + 16) + SCRATCH;
   static_assert(HEAD <= STAGES * STAGE, "a part fits the ring of a warp");
 };
 
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DecCfg<D, KIND, NT>::CTAS)
   extern __shared__ __align__(128) uint8_t smem[];
   float2* part_ml = reinterpret_cast<float2*>(smem + C::RING + C::HEADS);                  // [part][head]
   DecPart* parts = reinterpret_cast<DecPart*>(smem + C::RING + C::HEADS + C::PARTS * NH * 8);  // [part]
-  int* sh_sum = reinterpret_cast<int*>(parts + C::PARTS);                                  // [warp]
+  int* sh_sum = reinterpret_cast<int*>(parts + C::PARTS);                                  // [warp], room for two each
   int4* sh_at = reinterpret_cast<int4*>(sh_sum + 2 * DEC_WARPS);  // [warp] where its piece begins: sequence, length, head group, tile
   const tb200_attention_decode_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
