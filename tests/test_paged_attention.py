@@ -874,7 +874,7 @@ def test_argument_checks(cuda):
         varlen(k=kv.clone().requires_grad_())
     cos, sin = tables(64, 128, cuda)
     for bad in (dict(k=kv[:1], v=kv[:1]), dict(cos=cos), dict(cos=cos.double(), sin=sin.double()), dict(cos=cos[:, :4], sin=sin[:, :4]),
-                dict(cu_seqlens=cu[:2]), dict(q=torch.zeros(3, 8, 128, dtype=BF16, device=cuda)), dict(q_out=q[:1]), dict(k_out=q),
+                dict(cu_seqlens=cu[:2]), dict(q=None, q_out=q), dict(q=torch.zeros(3, 8, 128, dtype=BF16, device=cuda)), dict(q_out=q[:1]), dict(k_out=q),
                 dict(k_cache=cache.k[:, :, :1], v_cache=cache.v[:, :, :1])):
         with pytest.raises(AssertionError):
             append(**bad)

@@ -211,6 +211,7 @@ def append_paged_kv(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens=
         cos, sin = _aligned(cos), _aligned(sin)
         positions, half = cos.shape
         assert 0 < 2 * half <= d and half % 8 == 0, "rotary_dim: a multiple of 16, at most head_dim"
+    assert q is not None or q_out is None, "q_out without q"
     qo, qos, qoh = (None, 0, 0) if q is None else _out_rows(q_out, q, "q_out")
     ko, kos, koh = (None, 0, 0) if k_out is None else _out_rows(k_out, k, "k_out")
     q, qs, qh = (None, 0, 0) if q is None else _in_rows(q)
