@@ -328,7 +328,8 @@ int tb200_kv_append(const tb200_kv_append_args* args, void* stream);
  * log-sum-exp of the scaled scores. A sequence of length 0 gives o = 0 and lse = -inf.
  * q, o: [batch][heads][head_dim] with element strides (multiples of 8; bases 16-byte aligned). Caches 16-byte aligned with
  * strides that are multiples of 16 bytes. head_dim 64, 128 or 256; dtype TB200_BF16 or TB200_F16; sm_scale > 0;
- * max_pages * page_size at most 2^30 and batch * kv_heads * ceil(heads / kv_heads / 8) * max_pages * page_size / 16 below 2^31.
+ * max_pages * page_size at most 2^30 and batch * kv_heads * ceil(heads / kv_heads / 8) * max_pages * page_size / 16 below
+ * 2^31.
  * workspace: tb200_attention_decode_workspace_bytes(args) bytes, 16-byte aligned, contents free before and after; calls that
  * may run at the same time need workspaces of their own.
  */
@@ -366,9 +367,10 @@ int tb200_attention_decode(const tb200_attention_decode_args* args, void* stream
  * No sequence's output depends on the rows of another, whatever those hold; a NaN or infinity in v makes the rows of its
  * own sequence undefined, those that the mask keeps from it included (0 * inf).
  * head_dim 64, 128 or 256; dtype TB200_BF16 or TB200_F16; sm_scale > 0; bases 16-byte aligned, strides (elements, at least
- * head_dim) multiples of 8; tokens and max_pages * page_size at most 2^30 (the walk of one tile over its keys has to end
- * within the bound of a device-side wait, which is about 10^8 keys). workspace: tb200_attention_varlen_workspace_bytes(args) bytes, 32-byte aligned, contents free
- * before and after; calls that may run at the same time need workspaces of their own.
+ * head_dim) multiples of 8; tokens_q at most 2^30, tokens_k and max_pages * page_size at most 2^25 (the walk of one tile
+ * over its keys has to end within the bound of a device-side wait), TB200_ERR_UNSUPPORTED above. workspace:
+ * tb200_attention_varlen_workspace_bytes(args) bytes, 32-byte aligned, contents free before and after; calls that may run
+ * at the same time need workspaces of their own.
  */
 typedef struct {
   const void* q;

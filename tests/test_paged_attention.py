@@ -824,7 +824,8 @@ def test_decode_refusals(lib, change, code):
     (dict(q=None), -1), (dict(cu_seqlens_q=None), -1), (dict(seq_lens=None), -1), (dict(page_size=0, cu_seqlens_k=None), -1),
     (dict(heads=9), -1), (dict(page_size=12), -2), (dict(page_size=-1), -1), (dict(head_dim=32), -2), (dict(dtype=3), -2),
     (dict(sm_scale=-1.0), -1), (dict(v=4104), -1), (dict(k_stride_head=64), -1), (dict(q_stride_tok=1004), -1),
-    (dict(tokens_q=1 << 40), -2), (dict(workspace=None), -1), (dict(workspace_bytes=8), -1), (dict(workspace=4112), -1),
+    (dict(tokens_q=1 << 40), -2), (dict(max_pages=(1 << 21) + 1), -2), (dict(max_pages=1 << 62), -2),
+    (dict(page_size=0, tokens_k=(1 << 25) + 1), -2), (dict(workspace=None), -1), (dict(workspace_bytes=8), -1), (dict(workspace=4112), -1),
     (dict(tokens_q=0), 0), (dict(batch=0), 0)])
 def test_varlen_refusals(lib, change, code):
     from triton_b200 import _lib

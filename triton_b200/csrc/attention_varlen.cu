@@ -51,6 +51,9 @@ struct __align__(16) VarSplit {
   int tok0, n_tok, part, n_parts;
 };
 static constexpr int VAR_MIN_BLOCKS = 4;  // no piece is cut below this many KV blocks: starting one costs about two
+// Longest walk: a producer that is done waits for the whole of it, and a wait ends after 2 s. 2^25 keys are 2^18 blocks of
+// about 3400 cycles (128 x 2 queries, D = 128), 0.5 s at 1.9 GHz.
+static constexpr int VAR_MAX_KEYS = 1 << 25;
 struct VarCounters {
   int n_pieces, n_split, next, pad;
 };
@@ -995,8 +998,8 @@ extern "C" int tb200_attention_varlen_fwd(const tb200_attention_varlen_args* a, 
                              paged ? a->k_stride_page : a->k_stride_tok, paged ? a->v_stride_page : a->v_stride_tok};
   for (int64_t s : strides)
     if (s % 8 || s < a->head_dim) return TB200_ERR_BAD_ARG;
-  if (a->tokens_q > (1 << 30) || a->tokens_k > (1 << 30) || a->batch > (1 << 30) || a->heads > (1 << 16) ||
-      a->n_pages > (1 << 30) || a->max_pages > (1 << 30) || a->max_pages * a->page_size > (1 << 30))
+  if (a->tokens_q > (1 << 30) || a->tokens_k > VAR_MAX_KEYS || a->batch > (1 << 30) || a->heads > (1 << 16) ||
+      a->n_pages > (1 << 30) || (paged && (a->max_pages > VAR_MAX_KEYS || a->max_pages * a->page_size > VAR_MAX_KEYS)))
     return TB200_ERR_UNSUPPORTED;
   if (a->tokens_q == 0 || a->batch == 0 || a->heads == 0) return TB200_OK;
   if (!a->q || !a->o || !a->cu_seqlens_q) return TB200_ERR_BAD_ARG;

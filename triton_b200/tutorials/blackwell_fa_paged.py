@@ -23,8 +23,9 @@ Conventions:
 * ``page_table`` int32 ``[batch, max_pages]``: position p of sequence b lies in page ``page_table[b, p // page_size]``.
   ``seq_lens`` int32 ``[batch]``: tokens of each sequence in the cache, those of this call included. ``cu_seqlens`` int32
   ``[batch + 1]``: where each sequence's rows begin in the packed tensors. All of them stay on the device: no call
-  synchronises, so every call can be captured into a CUDA graph and replayed with other lengths. A length beyond the page
-  table is cut to it; a page outside the pool is never accessed, it reads as zeros and is not written.
+  synchronises, so every call can be captured into a CUDA graph and replayed with other lengths. Page tables of up to 2^30
+  tokens a sequence (prompts: 2^25 keys) are read. A length beyond the page table is cut to it;
+  a page outside the pool is never accessed, it reads as zeros and is not written.
 * ``out`` (``q_out``, ``k_out``): where results go; rows outside every sequence are left as they were (in a tensor that the
   call allocates: uninitialised). Outputs of the attention calls must not overlap their inputs.
 """
