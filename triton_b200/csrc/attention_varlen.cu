@@ -599,11 +599,11 @@ __global__ void __launch_bounds__(VAR_THREADS, 1) attention_varlen_kernel(const 
           if (!issue_pv(0, vcur, j > 0 ? 1u : 0u, iph0, mbar_test_a(p_full + 8 * 3, iph0), !more0)) { ok = false; break; }
           if (!k_ready && !var_wait(kv_full + 8 * knext, knext_ph, status, WAIT_SMEM_FULL)) { ok = false; break; }
           tc_fence_after_sync();
-          const bool p1_ready = both && mbar_test_a(p_full + 8 * 7, iph1);
           if (more0) {
             issue_qk(0, knext);
             if (j + 2 == n0) umma_commit_a(q_empty);
           }
+          const bool p1_ready = both && mbar_test_a(p_full + 8 * 7, iph1);
           if (both) {
             if (j == 0 && !var_wait(o_free + 8, tph1 ^ 1, status, WAIT_ATTN)) { ok = false; break; }
             if (!issue_pv(1, vcur, j > 0 ? 1u : 0u, iph1, p1_ready, false)) { ok = false; break; }
