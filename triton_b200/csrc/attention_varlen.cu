@@ -22,7 +22,7 @@
 //             page each. A page outside the pool is loaded from behind its end, which reads as zeros.
 // Bound: the chain scores -> softmax -> P V of a group, 3400 cycles per 128 keys at D = 128 (of them 1790 softmax, 1024
 // exponentials at the special-function unit's rate); tensor pipe about 60 %. Measured: 16001-token prompt, 32 / 8 heads of
-// 128, 1226 TFLOP/s from cold, 1075 under the power limit; 24 prompts of 5 to 3000 tokens 241 us = 0.58 of the floor.
+// 128, 1226 TFLOP/s from cold, 1075 under the power limit; 24 prompts of 5 to 3000 tokens 240 us = 0.58 of the floor.
 #include <limits.h>
 #include <string.h>
 
