@@ -328,8 +328,8 @@ int tb200_kv_append(const tb200_kv_append_args* args, void* stream);
  * log-sum-exp of the scaled scores. A sequence of length 0 gives o = 0 and lse = -inf.
  * q, o: [batch][heads][head_dim] with element strides (multiples of 8; bases 16-byte aligned). Caches 16-byte aligned with
  * strides that are multiples of 16 bytes. head_dim 64, 128 or 256; dtype TB200_BF16 or TB200_F16; sm_scale > 0;
- * max_pages * page_size at most 2^30 and batch * kv_heads * ceil(heads / kv_heads / 8) * max_pages * page_size / 16 below
- * 2^31.
+ * max_pages * page_size at most 2^30 and batch * kv_heads * ceil(heads / kv_heads / 8) * ceil(max_pages * page_size / 16)
+ * below 2^31 - 2^26, TB200_ERR_UNSUPPORTED otherwise.
  * workspace: tb200_attention_decode_workspace_bytes(args) bytes, 16-byte aligned, contents free before and after; calls that
  * may run at the same time need workspaces of their own.
  */

@@ -814,7 +814,8 @@ def test_append_refusals(lib, change, code):
     (dict(q=None), -1), (dict(seq_lens=None), -1), (dict(heads=7), -1), (dict(kv_heads=0), -1), (dict(page_size=0), -1),
     (dict(head_dim=32), -2), (dict(dtype=3), -2), (dict(cache_dtype=1), -2), (dict(cache_dtype=3, v_scale=None), -1),
     (dict(cache_dtype=3, kc_stride_tok=1032), -1), (dict(sm_scale=0.0), -1), (dict(sm_scale=float("nan")), -1), (dict(o=4098), -1),
-    (dict(q_stride_b=1001), -1), (dict(batch=0), 0), (dict(max_pages=1 << 40), -2), (dict(batch=1 << 40), -2)])
+    (dict(q_stride_b=1001), -1), (dict(batch=0), 0), (dict(max_pages=1 << 40), -2), (dict(batch=1 << 40), -2),
+    (dict(batch=(1 << 30) - (1 << 21), max_pages=1, heads=2), -2), (dict(batch=1 << 7, max_pages=1 << 23, heads=2), -2)])
 def test_decode_refusals(lib, change, code):
     from triton_b200 import _lib
     assert lib.tb200_attention_decode(ctypes.byref(filled(_lib.AttentionDecodeArgs, **change)), None) == code

@@ -738,9 +738,10 @@ struct DecPlan {
 };
 // A group of 8 query heads fills the narrow side of the mma; 16 per group halve the reads of K and V for larger groups
 // (head dim 256 keeps 8: two accumulators of 256 columns do not fit the registers).
+static int dec_heads(const tb200_attention_decode_args* a) { return a->heads / a->kv_heads > 8 && a->head_dim <= 128 ? 16 : 8; }
 static DecPlan dec_plan(const tb200_attention_decode_args* a, int sms) {
   DecPlan d;
-  d.nh = a->heads / a->kv_heads > 8 && a->head_dim <= 128 ? 16 : 8;
+  d.nh = dec_heads(a);
   d.ctas = sms * (a->head_dim == 256 ? 1 : 2);
   const size_t parts = (size_t)d.ctas * 2 * d.nh;
   d.off_warp = parts * a->head_dim * sizeof(float);
@@ -789,6 +790,11 @@ static int dec_check(const tb200_attention_decode_args* a) {
       a->n_pages > INT32_MAX ||
       a->max_pages * a->page_size > (1 << 30))
     return TB200_ERR_UNSUPPORTED;
+  // The kernel's positions on the line of tiles are 32-bit, and the end of a CTA's piece is computed before it is cut to the
+  // line's: up to 4 / 592 of the line behind it (4 warps a CTA, at least 148 CTAs), which 2^26 covers.
+  const int64_t nh = dec_heads(a), hgs = (a->heads / a->kv_heads + nh - 1) / nh * a->kv_heads;
+  const int64_t tiles = (a->max_pages * a->page_size + 15) / 16;  // of one sequence and head group, at most
+  if (hgs * tiles > INT32_MAX || a->batch * (hgs * tiles) > INT32_MAX - (1 << 26)) return TB200_ERR_UNSUPPORTED;
   return TB200_OK;
 }
 
@@ -826,9 +832,7 @@ extern "C" int tb200_attention_decode(const tb200_attention_decode_args* a, void
   const int sms = sm_count();
   if (sms <= 0) return TB200_ERR_CUDA;
   const DecPlan plan = dec_plan(a, sms);
-  const int64_t group = a->heads / a->kv_heads, hgs = (group + plan.nh - 1) / plan.nh * a->kv_heads;
-  const int64_t tiles = (a->max_pages * a->page_size + 15) / 16;  // of one sequence and head group, at most
-  if (plan.ctas > 1024 || hgs * tiles > INT32_MAX || a->batch * (hgs * tiles) > INT32_MAX - (1 << 20)) return TB200_ERR_UNSUPPORTED;
+  if (plan.ctas > 1024) return TB200_ERR_UNSUPPORTED;
   if (!a->workspace || off16(a->workspace) || a->workspace_bytes < plan.bytes) return TB200_ERR_BAD_ARG;
   DecodeParams p;
   memset(&p, 0, sizeof(p));
